@@ -518,6 +518,82 @@ KANI_API int kani_codec_codes(const int64_t* tokens, int64_t tokens_row_stride, 
                      int64_t codebook_size, int64_t* codes_out, int64_t max_frames,
                      int64_t* frames_out, int32_t* status_out, void* stream);
 
+/*
+ * GQA decode attention of a batch of streams that share a long prefix: one query
+ * per stream over the prefix rows and then the stream's own valid cache rows,
+ *   out[b, hq, :] = sum_j w_j v_j,  w = softmax_j(scale * q[b, hq, :] . k_j),
+ * j over prefix rows [0, *prefix_len) (prefix_len NULL: all prefix_rows) and own
+ * rows [0, kv_len[b]); a query without any row gets zeros.  kani_decode_attention's
+ * operation when prefix_rows is 0.  The prefix is read once for the whole batch.
+ * With scores not NULL, scores[b, h, j] += sum over the heads of KV head h of their
+ * weight w_j on own row j (fp32; the running weight that kani_cache_evict keeps by).
+ *   q, out: [batch, Hq, D] (batch / head strides); caches [batch, Hk, cache_len, D]
+ *   (strides, a last dimension of stride 1); prefix_k, prefix_v [Hk, prefix_rows, D];
+ *   scores [batch, Hk, cache_len]; kv_len, prefix_len: device int64.
+ *   bf16 / fp16; D = 64 or 128; Hq / Hk at most 8; 16-byte aligned rows; scale >= 0.
+ *   A length outside its range is held to it and sets KANI_FLAG_SLOT_OOB.
+ *   workspace: device scratch of kani_prefix_decode_workspace(...) bytes (256-byte
+ *   aligned; NULL when that is 0), which no other call may use at the same time.
+ */
+KANI_API int64_t kani_prefix_decode_workspace(int64_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                     int32_t head_dim, int64_t cache_len, int64_t prefix_rows, int32_t with_scores);
+KANI_API int kani_prefix_decode_attention(int32_t dtype, int64_t batch, int32_t num_q_heads,
+                     int32_t num_kv_heads, int32_t head_dim, const void* q, int64_t q_batch_stride,
+                     int64_t q_head_stride, const void* k_cache, const void* v_cache,
+                     int64_t cache_batch_stride, int64_t cache_head_stride, int64_t cache_slot_stride,
+                     int64_t cache_len, const int64_t* kv_len, const void* prefix_k, const void* prefix_v,
+                     int64_t prefix_head_stride, int64_t prefix_row_stride, int64_t prefix_rows,
+                     const int64_t* prefix_len, float scale, float* scores, int64_t scores_batch_stride,
+                     int64_t scores_head_stride, void* out, int64_t out_batch_stride,
+                     int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
+                     int32_t* err_flag, void* stream);
+
+/*
+ * The prompt pass of the same attention: query i < q_len[b] of stream b (q_len NULL:
+ * all tokens) is the stream's own cache row kv_len[b] - q_len[b] + i and sees the
+ * prefix rows and its own rows up to that one; queries from q_len[b] on get zeros.
+ *   q, out: [batch, tokens, Hq, D] (batch / token / head strides); everything else,
+ *   the workspace (kani_prefix_prefill_workspace) included, as above.
+ *   kv_len[b] < q_len[b] sets KANI_FLAG_SLOT_OOB (query i is then own row i).
+ */
+KANI_API int64_t kani_prefix_prefill_workspace(int64_t batch, int64_t tokens, int32_t num_q_heads,
+                     int32_t num_kv_heads, int32_t head_dim, int64_t cache_len, int64_t prefix_rows);
+KANI_API int kani_prefix_prefill_attention(int32_t dtype, int64_t batch, int64_t tokens,
+                     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, const void* q,
+                     int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                     const void* k_cache, const void* v_cache, int64_t cache_batch_stride,
+                     int64_t cache_head_stride, int64_t cache_slot_stride, int64_t cache_len,
+                     const int64_t* kv_len, const int64_t* q_len, const void* prefix_k,
+                     const void* prefix_v, int64_t prefix_head_stride, int64_t prefix_row_stride,
+                     int64_t prefix_rows, const int64_t* prefix_len, float scale, void* out,
+                     int64_t out_batch_stride, int64_t out_token_stride, int64_t out_head_stride,
+                     void* workspace, int64_t workspace_bytes, int32_t* err_flag, void* stream);
+
+/*
+ * Eviction from static caches by accumulated attention weight.  A stream of
+ * n = kv_len[b] > budget rows keeps, per KV head h, its first `protect` rows, its
+ * last `recent` rows and, of the rows between, the budget - protect - recent with
+ * the highest scores[b, h, j] (ties: the lowest slot; NaN counts as the lowest
+ * score); other streams keep all rows.  Kept rows move in slot order to rows
+ * [0, min(n, budget)) of k_out / v_out / scores_out: the caches and scores
+ * themselves (all three the same pointers, strides and out_len), or buffers that
+ * do not overlap them.  scores_out rows past the new length become zero, K / V rows
+ * past it stay as they were.  len_out[b] = min(n, budget) (not kv_len itself);
+ * kept_out [batch, Hk, budget] int32 (may be NULL): the kept slots, then -1.
+ *   caches [batch, Hk, cache_len, D], outputs [batch, Hk, out_len, D] (strides, rows
+ *   of a multiple of 16 bytes, 16-byte aligned, D <= 256); fp32 / bf16 / fp16;
+ *   protect + recent <= budget <= out_len.
+ */
+KANI_API int kani_cache_evict(int32_t dtype, int64_t batch, int32_t num_kv_heads, int32_t head_dim,
+                     const void* k_cache, const void* v_cache, int64_t cache_batch_stride,
+                     int64_t cache_head_stride, int64_t cache_slot_stride, int64_t cache_len,
+                     const float* scores, int64_t scores_batch_stride, int64_t scores_head_stride,
+                     const int64_t* kv_len, int64_t budget, int64_t recent, int64_t protect,
+                     void* k_out, void* v_out, int64_t out_batch_stride, int64_t out_head_stride,
+                     int64_t out_slot_stride, int64_t out_len, float* scores_out,
+                     int64_t scores_out_batch_stride, int64_t scores_out_head_stride, int64_t* len_out,
+                     int32_t* kept_out, int32_t* err_flag, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

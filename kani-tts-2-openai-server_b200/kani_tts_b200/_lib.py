@@ -95,6 +95,21 @@ _SIGNATURES = {
                            _c_p, _c_p], ctypes.c_int),
     "kani_codec_codes": ([_c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p,
                           _c_p], ctypes.c_int),
+    "kani_prefix_decode_workspace": ([_c_i64, _c_i32, _c_i32, _c_i32, _c_i64, _c_i64, _c_i32], _c_i64),
+    "kani_prefix_decode_attention": ([_c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_i64, _c_i64,
+                                      _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p,
+                                      _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_f32,
+                                      _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p],
+                                     ctypes.c_int),
+    "kani_prefix_prefill_workspace": ([_c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i64, _c_i64], _c_i64),
+    "kani_prefix_prefill_attention": ([_c_i32, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_i64, _c_i64, _c_i64,
+                                       _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p,
+                                       _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_f32,
+                                       _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p], ctypes.c_int),
+    "kani_cache_evict": ([_c_i32, _c_i64, _c_i32, _c_i32, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64,
+                          _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64,
+                          _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p,
+                          _c_p, _c_p, _c_p], ctypes.c_int),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

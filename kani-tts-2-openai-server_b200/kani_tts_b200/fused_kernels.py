@@ -8,7 +8,10 @@ Same names, argument meaning and return values as the reference module
   folded into the following RMSNorm;
 * ``kv_cache_write`` — the scatter_ of static_cache.py:131-140;
 * ``fused_rope_kv_write`` — q/k norm + cos/sin + RoPE (+ BemaTTS frame term)
-  + KV write of optimized_decode.py:220-240 in one launch.
+  + KV write of optimized_decode.py:220-240 in one launch;
+* ``prefix_decode_attention`` / ``prefix_prefill_attention`` — attention of a batch of
+  streams that share a long prefix, and ``evict_cache`` — eviction from the static
+  caches by accumulated attention weight.
 
 Each call validates its tensors on the host (device, dtype, shape) before a
 single launch through the C ABI on the current CUDA stream; nothing
@@ -25,6 +28,8 @@ the reference, all deliberate:
 """
 from __future__ import annotations
 
+import contextlib
+import functools
 import math
 
 import torch
@@ -52,6 +57,9 @@ __all__ = [
     "gemv_short_conv",
     "decode_advance",
     "gemv_rope_kv_write",
+    "prefix_decode_attention",
+    "prefix_prefill_attention",
+    "evict_cache",
 ]
 
 
@@ -1056,6 +1064,303 @@ def codec_codes(tokens: torch.Tensor, eos_token: int, audio_tokens_start: int, c
                                int(codebook_size), ptr(codes), mf, ptr(frames), ptr(status), stream_ptr(dev)),
           "kani_codec_codes")
     return codes, frames, status
+
+
+def _on_one_device(dev: torch.device, named) -> None:
+    """Every given tensor must be a CUDA tensor on `dev` (None is skipped)."""
+    for t, w in named:
+        if t is not None:
+            require_cuda(t, w)
+            if t.device != dev:
+                raise ValueError(f"{w} is on {t.device}, q or the cache on {dev}")
+
+
+def _launch_on(dev: torch.device):
+    """Makes `dev` the current device for a launch on its stream, where it is not."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """Byte addresses [first, past the last) that a tensor's elements lie in."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _refuse_overlap(out: torch.Tensor, what: str, named) -> None:
+    """An output that a call writes while it still reads others must lie apart from them."""
+    a0, a1 = _span(out)
+    for t, w in named:
+        if t is not None:
+            b0, b1 = _span(t)
+            if a0 < b1 and b0 < a1:
+                raise ValueError(f"{what} must not overlap {w}")
+    if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
+        raise ValueError(f"{what} must not be an expanded view")
+
+
+def _lengths(t: torch.Tensor, n: int, what: str) -> torch.Tensor:
+    if t.dtype != torch.int64 or t.numel() != n:
+        raise ValueError(f"{what} must be int64 with {n} element{'s' if n != 1 else ''}")
+    return t.contiguous()
+
+
+def _shared_prefix(prefix_k, prefix_v, prefix_len, q, hk: int, d: int):
+    """The prefix as (k, v, rows, head stride, row stride, length); no prefix: zero rows."""
+    if prefix_k is None or prefix_v is None:
+        if prefix_k is not prefix_v or prefix_len is not None:
+            raise ValueError("prefix_k and prefix_v must be given together, and prefix_len only with them")
+        return None, None, 0, 0, 0, None
+    if prefix_k.dim() == 4 and prefix_k.shape[0] == 1:
+        prefix_k = prefix_k[0]
+    if prefix_v.dim() == 4 and prefix_v.shape[0] == 1:
+        prefix_v = prefix_v[0]
+    if prefix_k.dim() != 3 or prefix_k.shape[0] != hk or prefix_k.shape[2] != d or prefix_v.shape != prefix_k.shape:
+        raise ValueError(f"prefix_k / prefix_v must both be [{hk}, rows, {d}], got {tuple(prefix_k.shape)} / "
+                         f"{tuple(prefix_v.shape)}")
+    if prefix_k.dtype != q.dtype or prefix_v.dtype != q.dtype:
+        raise TypeError("the prefix must have the dtype of q")
+    st = prefix_k.stride()
+    if st != prefix_v.stride() or st[2] != 1:
+        raise ValueError("prefix_k and prefix_v need the same strides with a contiguous last dim")
+    plen = None if prefix_len is None else _lengths(prefix_len, 1, "prefix_len")
+    return prefix_k, prefix_v, prefix_k.shape[1], st[0], st[1], plen
+
+
+def _own_cache(k_cache, v_cache, q):
+    """Checked sizes and strides of a [B, Hk, S, D] cache pair."""
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("k_cache / v_cache must both be [batch, kv_heads, max_len, head_dim]")
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise TypeError("q and the caches must share one dtype")
+    st = k_cache.stride()
+    if st != v_cache.stride() or (st[3] != 1 and k_cache.numel()):
+        raise ValueError("k_cache and v_cache need the same strides with a contiguous last dim")
+    return k_cache.shape, st
+
+
+def _attention_scale(scale, d: int) -> float:
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 <= scale < math.inf:
+        raise ValueError(f"scale must be finite and not negative, got {scale}")
+    return scale
+
+
+@functools.lru_cache(maxsize=1024)
+def _prefix_workspace_bytes(entry: str, device_index: int, *sizes: int) -> int:
+    return int(getattr(load_library(), entry)(*sizes))
+
+
+def _workspace(entry: str, dev: torch.device, *sizes: int):
+    """A call's device scratch.  It comes from the caching allocator on the current
+    stream (inside a capture from the graph's own pool), so calls on other streams
+    and other graphs never share it."""
+    n = _prefix_workspace_bytes(entry, dev.index, *sizes)
+    return (torch.empty(n, dtype=torch.uint8, device=dev) if n else None), n
+
+
+def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor,
+                            prefix_k: torch.Tensor | None = None, prefix_v: torch.Tensor | None = None,
+                            prefix_len: torch.Tensor | None = None, *, scale: float | None = None,
+                            scores: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                            err_flag: torch.Tensor | None = None) -> torch.Tensor:
+    """GQA decode attention of streams that share a prefix (``kani_prefix_decode_attention``).
+
+    One query token per stream attends to the prefix rows, which all streams share
+    and which are read once for the batch, and to its own cache slots [0, kv_len[b]):
+    ``decode_attention`` over the concatenation of both (optimized_decode.py:243-248
+    with the prefix copied into every stream's buffer).
+
+    Args:
+        q: [B, Hq, D] or [B, 1, Hq, D] (contiguous last dim); D 64 or 128, bf16 / fp16.
+        k_cache / v_cache: [B, Hk, S, D], equal strides; Hq / Hk at most 8.
+        kv_len: device int64 [B]; 0 is allowed.
+        prefix_k / prefix_v: [Hk, P, D] (or [1, Hk, P, D]); None = no prefix.
+        prefix_len: device int64 [1], rows of the prefix in use (default: all P).
+        scores: optional fp32 [B, Hk, S]; each own row's weight, summed over the query
+            heads of its KV head, is added to it (the running weight ``evict_cache``
+            keeps by).
+        out: optional contiguous output of B * Hq * D elements.
+    Returns out [B, Hq, D]; zeros where a stream sees no row at all.  A length out of
+    range is held to it and flagged in ``err_flag``.
+    """
+    dev = q.device
+    _on_one_device(dev, ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (kv_len, "kv_len"),
+                         (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (prefix_len, "prefix_len"),
+                         (scores, "scores"), (out, "out"), (err_flag, "err_flag")))
+    lib = load_library()
+    code = dtype_code(q, "q")
+    (b, hk, s_len, d), cs = _own_cache(k_cache, v_cache, q)
+    qv = q.squeeze(1) if q.dim() == 4 and q.shape[1] == 1 else q
+    if qv.dim() != 3 or qv.shape[0] != b or qv.shape[2] != d or (qv.stride(2) != 1 and qv.numel()):
+        raise ValueError(f"q must be [{b}, heads, {d}] with a contiguous last dim")
+    hq = qv.shape[1]
+    if hk == 0 or hq % hk:
+        raise ValueError(f"{hq} query heads do not group over {hk} KV heads")
+    kv_len = _lengths(kv_len, b, "kv_len")
+    pk, pv, rows, ph, ps, plen = _shared_prefix(prefix_k, prefix_v, prefix_len, q, hk, d)
+    scale = _attention_scale(scale, d)
+    sb = sh = 0
+    if scores is not None:
+        if scores.dtype != torch.float32 or scores.shape != (b, hk, s_len) or (scores.stride(2) != 1 and s_len > 1):
+            raise ValueError(f"scores must be fp32 [{b}, {hk}, {s_len}] with a contiguous last dim")
+        sb, sh = scores.stride()[:2]
+        _refuse_overlap(scores, "scores", ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (out, "out")))
+    if out is None:
+        out = torch.empty(b, hq, d, dtype=q.dtype, device=dev)
+    else:
+        if out.numel() != b * hq * d or out.dtype != q.dtype or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {q.dtype} tensor of {b * hq * d} elements")
+        _refuse_overlap(out, "out", ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (pk, "prefix_k"),
+                                     (pv, "prefix_v")))
+    flag = err_flag if err_flag is not None else error_flag(dev)
+    with _launch_on(dev):
+        ws, n = _workspace("kani_prefix_decode_workspace", dev, b, hq, hk, d, s_len, rows, int(scores is not None))
+        check(lib.kani_prefix_decode_attention(
+            code, b, hq, hk, d, qv.data_ptr(), qv.stride(0), qv.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
+            cs[0], cs[1], cs[2], s_len, kv_len.data_ptr(), ptr(pk), ptr(pv), ph, ps, rows, ptr(plen), scale,
+            ptr(scores), sb, sh, out.data_ptr(), hq * d, d, ptr(ws), n, flag.data_ptr(),
+            torch.cuda.current_stream(dev).cuda_stream), "kani_prefix_decode_attention")
+    return out
+
+
+def prefix_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor,
+                             prefix_k: torch.Tensor | None = None, prefix_v: torch.Tensor | None = None,
+                             prefix_len: torch.Tensor | None = None, *, q_len: torch.Tensor | None = None,
+                             scale: float | None = None, out: torch.Tensor | None = None,
+                             err_flag: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal GQA attention of prompt tokens that follow a shared prefix
+    (``kani_prefix_prefill_attention``): the prefill's SDPA (the HF prompt pass,
+    inference_engine.py:475-500) with the prefix rows in front, without repeating
+    K / V heads and with a length per stream.
+
+    Args:
+        q: [B, T, Hq, D] (contiguous last dim).
+        k_cache / v_cache: [B, Hk, S, D]: the rows of these tokens are in them already.
+        kv_len: device int64 [B], valid own rows including these tokens'.
+        q_len: device int64 [B], real tokens of each stream's T (default: all T).
+            Token i < q_len[b] is own row kv_len[b] - q_len[b] + i and sees the prefix
+            and its own rows up to that one; later tokens' outputs are zeros.
+        prefix_k, prefix_v, prefix_len, scale, err_flag: as in
+            ``prefix_decode_attention``.  out: optional contiguous [B, T, Hq, D].
+    Returns out [B, T, Hq, D].
+    """
+    dev = q.device
+    _on_one_device(dev, ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (kv_len, "kv_len"), (q_len, "q_len"),
+                         (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (prefix_len, "prefix_len"), (out, "out"),
+                         (err_flag, "err_flag")))
+    lib = load_library()
+    code = dtype_code(q, "q")
+    (b, hk, s_len, d), cs = _own_cache(k_cache, v_cache, q)
+    if q.dim() != 4 or q.shape[0] != b or q.shape[3] != d or (q.stride(3) != 1 and q.numel()):
+        raise ValueError(f"q must be [{b}, tokens, heads, {d}] with a contiguous last dim")
+    t, hq = q.shape[1:3]
+    if hk == 0 or hq % hk:
+        raise ValueError(f"{hq} query heads do not group over {hk} KV heads")
+    kv_len = _lengths(kv_len, b, "kv_len")
+    q_len = None if q_len is None else _lengths(q_len, b, "q_len")
+    pk, pv, rows, ph, ps, plen = _shared_prefix(prefix_k, prefix_v, prefix_len, q, hk, d)
+    scale = _attention_scale(scale, d)
+    if out is None:
+        out = torch.empty(b, t, hq, d, dtype=q.dtype, device=dev)
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)}")
+        _refuse_overlap(out, "out", ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (pk, "prefix_k"),
+                                     (pv, "prefix_v")))
+    flag = err_flag if err_flag is not None else error_flag(dev)
+    qs = q.stride()
+    with _launch_on(dev):
+        ws, n = _workspace("kani_prefix_prefill_workspace", dev, b, t, hq, hk, d, s_len, rows)
+        check(lib.kani_prefix_prefill_attention(
+            code, b, t, hq, hk, d, q.data_ptr(), qs[0], qs[1], qs[2], k_cache.data_ptr(), v_cache.data_ptr(),
+            cs[0], cs[1], cs[2], s_len, kv_len.data_ptr(), ptr(q_len), ptr(pk), ptr(pv), ph, ps, rows, ptr(plen),
+            scale, out.data_ptr(), t * hq * d, hq * d, d, ptr(ws), n, flag.data_ptr(),
+            torch.cuda.current_stream(dev).cuda_stream), "kani_prefix_prefill_attention")
+    return out
+
+
+def evict_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor, kv_len: torch.Tensor, budget: int,
+                recent: int, protect: int = 0, *, k_out: torch.Tensor | None = None,
+                v_out: torch.Tensor | None = None, scores_out: torch.Tensor | None = None,
+                len_out: torch.Tensor | None = None, kept_out: torch.Tensor | None = None,
+                err_flag: torch.Tensor | None = None) -> torch.Tensor:
+    """Cut static caches down to `budget` rows by accumulated attention weight
+    (``kani_cache_evict``; the reference's static cache has no eviction and ends
+    generation at max_total_len, static_cache.py:110-142).
+
+    A stream with more than `budget` valid rows keeps, per KV head, its first
+    `protect` rows, its last `recent` rows and, of the others, those with the highest
+    ``scores`` (ties: the lowest slot; NaN counts as the lowest score), in slot order.
+    Keys carry their rotary angles, so kept rows need no change when they move.
+
+    Args:
+        k_cache / v_cache: [B, Hk, S, D], fp32 / bf16 / fp16, equal strides.
+        scores: fp32 [B, Hk, S] (``prefix_decode_attention``'s).
+        kv_len: device int64 [B], valid rows (unchanged; copy the result into it).
+        k_out / v_out / scores_out: destination buffers [B, Hk, S', D] / [B, Hk, S'],
+            S' >= budget, apart from the caches; all None: in place.
+        len_out: optional int64 [B] for the new lengths.
+        kept_out: optional int32 [B, Hk, budget]: the kept slots, then -1.
+    Returns the new lengths min(kv_len, budget), int64 [B].  Scores past the new
+    length become zero (the next rows start from there); K / V rows past it stay as
+    they were.
+    """
+    dev = k_cache.device
+    _on_one_device(dev, ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores"), (kv_len, "kv_len"),
+                         (k_out, "k_out"), (v_out, "v_out"), (scores_out, "scores_out"), (len_out, "len_out"),
+                         (kept_out, "kept_out"), (err_flag, "err_flag")))
+    lib = load_library()
+    code = dtype_code(k_cache, "k_cache")
+    (b, hk, s_len, d), cs = _own_cache(k_cache, v_cache, k_cache)
+
+    def check_scores(t, rows, what):
+        if t.dtype != torch.float32 or t.shape != (b, hk, rows) or (t.stride(2) != 1 and rows > 1):
+            raise ValueError(f"{what} must be fp32 [{b}, {hk}, {rows}] with a contiguous last dim")
+
+    check_scores(scores, s_len, "scores")
+    kv_len = _lengths(kv_len, b, "kv_len")
+    given = sum(t is not None for t in (k_out, v_out, scores_out))
+    if given not in (0, 3):
+        raise ValueError("k_out, v_out and scores_out must be given together (or none of them: in place)")
+    inputs = ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores"), (kv_len, "kv_len"))
+    if given:
+        (bo, hko, out_len, do), co = _own_cache(k_out, v_out, k_cache)
+        if (bo, hko, do) != (b, hk, d):
+            raise ValueError(f"k_out / v_out must be [{b}, {hk}, rows, {d}]")
+        check_scores(scores_out, out_len, "scores_out")
+        for t, w in ((k_out, "k_out"), (v_out, "v_out"), (scores_out, "scores_out")):
+            _refuse_overlap(t, w, inputs)
+    else:
+        k_out, v_out, scores_out, out_len, co = k_cache, v_cache, scores, s_len, cs
+        for t, w in ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores")):
+            _refuse_overlap(t, w, ((kv_len, "kv_len"),))
+    if k_out.data_ptr() == v_out.data_ptr() and k_out.numel():
+        raise ValueError("keys and values must be different tensors")
+    budget, recent, protect = int(budget), int(recent), int(protect)
+    if budget < 0 or recent < 0 or protect < 0 or protect + recent > budget or budget > out_len:
+        raise ValueError(f"0 <= protect + recent <= budget <= {out_len} expected, got protect {protect}, "
+                         f"recent {recent}, budget {budget}")
+    if len_out is None:
+        len_out = torch.empty(b, dtype=torch.int64, device=dev)
+    elif len_out.dtype != torch.int64 or len_out.numel() != b or not len_out.is_contiguous():
+        raise ValueError(f"len_out must be contiguous int64 with {b} elements")
+    else:
+        _refuse_overlap(len_out, "len_out", inputs)
+    if kept_out is not None:
+        if kept_out.dtype != torch.int32 or kept_out.shape != (b, hk, budget) or not kept_out.is_contiguous():
+            raise ValueError(f"kept_out must be contiguous int32 [{b}, {hk}, {budget}]")
+        _refuse_overlap(kept_out, "kept_out", inputs)
+    flag = err_flag if err_flag is not None else error_flag(dev)
+    ss, so = scores.stride(), scores_out.stride()
+    with _launch_on(dev):
+        check(lib.kani_cache_evict(
+            code, b, hk, d, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], s_len, scores.data_ptr(),
+            ss[0], ss[1], kv_len.data_ptr(), budget, recent, protect, k_out.data_ptr(), v_out.data_ptr(), co[0],
+            co[1], co[2], out_len, scores_out.data_ptr(), so[0], so[1], len_out.data_ptr(), ptr(kept_out),
+            flag.data_ptr(), torch.cuda.current_stream(dev).cuda_stream), "kani_cache_evict")
+    return len_out
 
 
 def launch_count() -> int:
