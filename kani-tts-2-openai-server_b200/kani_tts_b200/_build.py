@@ -23,7 +23,7 @@ LIB_PATH = LIB_DIR / "libkani_b200.so"
 
 SOURCES = ["capi.cu", "rms_norm.cu", "silu_mul.cu", "rope_kv.cu", "decode_attn.cu", "short_conv.cu",
            "sampling.cu", "head_argmax.cu", "codec_codes.cu", "gemv.cu",
-           "decode_advance.cu", "head_tc.cu", "gemm_tc.cu", "prefix_attn.cu", "cache_evict.cu"]
+           "decode_advance.cu", "head_tc.cu", "gemm_tc.cu", "prefix_decode.cu", "prefix_prefill.cu", "cache_evict.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
