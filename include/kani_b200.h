@@ -552,12 +552,10 @@ KANI_API int kani_prefix_decode_attention(int32_t dtype, int64_t batch, int32_t 
  * The prompt pass of the same attention: query i < q_len[b] of stream b (q_len NULL:
  * all tokens) is the stream's own cache row kv_len[b] - q_len[b] + i and sees the
  * prefix rows and its own rows up to that one; queries from q_len[b] on get zeros.
- *   q, out: [batch, tokens, Hq, D] (batch / token / head strides); everything else,
- *   the workspace (kani_prefix_prefill_workspace) included, as above.
+ *   q, out: [batch, tokens, Hq, D] (batch / token / head strides); everything else as
+ *   above, without a workspace.
  *   kv_len[b] < q_len[b] sets KANI_FLAG_SLOT_OOB (query i is then own row i).
  */
-KANI_API int64_t kani_prefix_prefill_workspace(int64_t batch, int64_t tokens, int32_t num_q_heads,
-                     int32_t num_kv_heads, int32_t head_dim, int64_t cache_len, int64_t prefix_rows);
 KANI_API int kani_prefix_prefill_attention(int32_t dtype, int64_t batch, int64_t tokens,
                      int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, const void* q,
                      int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
@@ -567,7 +565,7 @@ KANI_API int kani_prefix_prefill_attention(int32_t dtype, int64_t batch, int64_t
                      const void* prefix_v, int64_t prefix_head_stride, int64_t prefix_row_stride,
                      int64_t prefix_rows, const int64_t* prefix_len, float scale, void* out,
                      int64_t out_batch_stride, int64_t out_token_stride, int64_t out_head_stride,
-                     void* workspace, int64_t workspace_bytes, int32_t* err_flag, void* stream);
+                     int32_t* err_flag, void* stream);
 
 /*
  * Eviction from static caches by accumulated attention weight.  A stream of

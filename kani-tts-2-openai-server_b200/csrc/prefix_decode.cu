@@ -30,6 +30,7 @@
 #include <algorithm>
 
 #include "prefix_attn.cuh"
+#include "prefix_flash.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -43,11 +44,16 @@ using prefix::Params;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kMaxSlack = 8.f;             // the running maximum may lag by this many powers of 2
+constexpr int64_t kSharedBytes = 128 << 20;  // prefix bytes, times the streams, from which it is read once
 constexpr int64_t kLogitSmem = 32 * 1024;    // logits kept in shared memory up to this many bytes
 
 struct DecodeParams : Params {
-  float* logits;      // workspace [B, Hq, cache_len] when they do not fit in shared memory
-  int logit_rows;     // else rows per CTA
+  float* logits;     // workspace [B, Hq, cache_len] when they do not fit in shared memory
+  int logit_rows;    // else rows per CTA
+  int by_length;     // blocks take the streams in the order of their lengths
+  int parts;         // the prefix's partials (0: this kernel reads the prefix rows itself)
+  const float* acc;  // [parts][B, Hq][D]
+  const float* ml;   // [parts][B, Hq][2]
 };
 
 __device__ __forceinline__ uint32_t smem32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -104,6 +110,14 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint3
 template <int D, int KEYS, int STAGES>
 constexpr size_t kRingBytes = (size_t)kWarps * STAGES * 2 * KEYS * D * 2;
 
+// After the last row the rings are idle: each warp's holds its own partial first, and
+// in rank 0's the partials of the cluster's CTAs r = warp and r = warp + 4 behind it.
+template <int D>
+constexpr int kPartBytes = (8 * (D + 2) * 4 + 127) / 128 * 128;
+constexpr int kMaxParts = 16;  // of the prefix; 8 heads' factors of all partials fit the first slot
+template <int D>
+constexpr int kFirstSlot = kPartBytes<D> > 8 * (kMaxParts + 8) * 4 ? kPartBytes<D> : 8 * (kMaxParts + 8) * 4;
+
 template <typename T, int D, int KEYS, int STAGES>
 __global__ void __launch_bounds__(kThreads) prefix_decode_kernel(const __grid_constant__ DecodeParams p) {
   constexpr int ROW = D * 2;             // bytes
@@ -113,16 +127,41 @@ __global__ void __launch_bounds__(kThreads) prefix_decode_kernel(const __grid_co
   extern __shared__ __align__(128) unsigned char smem[];
   cg::cluster_group cluster = cg::this_cluster();
   const int ncl = (int)gridDim.x, rank = (int)blockIdx.x;
-  const int h = blockIdx.y, b = blockIdx.z, G = p.group;
+  const int h = blockIdx.y, G = p.group;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int b = blockIdx.z;
+  if (p.by_length) {
+    // blocks start in the order of z: the longest stream first, so that the last ones
+    // to start are short (64 streams of 120..1500 rows: 24.9 us against 30.8)
+    int* len = reinterpret_cast<int*>(smem);
+    __shared__ int s_b;
+    const int n = p.batch <= tid ? -1 : (int)min(max(p.kv_len[tid], (int64_t)0), p.cache_len);
+    len[tid] = n;
+    __syncthreads();
+    int before = 0;
+#pragma unroll 4
+    for (int j = 0; j < p.batch; j += 4) {
+      const int4 o = *reinterpret_cast<const int4*>(len + j);
+      before += (o.x > n || (o.x == n && j < tid)) + (o.y > n || (o.y == n && j + 1 < tid)) +
+                (o.z > n || (o.z == n && j + 2 < tid)) + (o.w > n || (o.w == n && j + 3 < tid));
+    }
+    if (n >= 0 && before == b) s_b = tid;
+    __syncthreads();
+    b = s_b;
+  }
   const int g = lane >> 2, t4 = lane & 3;  // this lane's head (row) and pair of columns in a product
-  float* gathered = reinterpret_cast<float*>(smem + kRingBytes<D, KEYS, STAGES>);  // [ncl][G][PART], rank 0's is used
-  float* stat = gathered + ncl * G * PART;                                           // [G][2]: m, 1 / l
-  float* s_logits = stat + 2 * G;                                                    // [G][logit_rows]
+  constexpr int WRING = STAGES * 2 * TILE;  // bytes of a warp's ring
+  static_assert(kFirstSlot<D> + 2 * kPartBytes<D> <= WRING, "the partials fit the rings");
+  auto gathered = [&](int r, int hd) {  // CTA r's partial of a head (rank 0's memory)
+    return reinterpret_cast<float*>(smem + (r & 3) * WRING + kFirstSlot<D> + (r >> 2) * kPartBytes<D>) + hd * PART;
+  };
+  float* stat = reinterpret_cast<float*>(smem + kRingBytes<D, KEYS, STAGES>);  // [G][2]: m, 1 / l
+  float* s_logits = stat + 2 * G;                                              // [G][logit_rows]
 
   const bool tell = rank == 0 && h == 0 && tid == 0;
-  const int plen = p.prefix_len ? prefix::checked_len(*p.prefix_len, p.prefix_rows, p.err, tell && b == 0)
-                                : (int)p.prefix_rows;
+  const int plen = p.parts        ? 0
+                   : p.prefix_len ? prefix::checked_len(*p.prefix_len, p.prefix_rows, p.err, tell && b == 0)
+                                  : (int)p.prefix_rows;
   const int own = prefix::checked_len(p.kv_len[b], p.cache_len, p.err, tell);
   // this CTA's rows: [p0, p0 + np) of the prefix, then [o0, o0 + no) of the stream
   const int pc = (plen + ncl - 1) / ncl, oc = (own + ncl - 1) / ncl;
@@ -139,7 +178,7 @@ __global__ void __launch_bounds__(kThreads) prefix_decode_kernel(const __grid_co
   const char* vo = reinterpret_cast<const char*>(static_cast<const T*>(p.v) + b * p.cb + h * p.ch + (int64_t)o0 * p.cs);
   const int64_t pstep = p.ps * 2, ostep = p.cs * 2;
 
-  const uint32_t ring = smem32(smem) + (uint32_t)warp * STAGES * 2 * TILE;
+  const uint32_t ring = smem32(smem) + (uint32_t)warp * WRING;
   const int rl = lane / CH, cl = lane % CH;
   auto issue = [&](int it) {
     const uint32_t kt = ring + (uint32_t)(it % STAGES) * 2 * TILE;
@@ -249,7 +288,7 @@ __global__ void __launch_bounds__(kThreads) prefix_decode_kernel(const __grid_co
 
   // this warp's partial, into its own (now idle) ring
   __syncwarp();
-  float* mine = reinterpret_cast<float*>(smem + (size_t)warp * STAGES * 2 * TILE);
+  float* mine = reinterpret_cast<float*>(smem + (size_t)warp * WRING);
   if (g < G) {
     float* w = mine + g * PART;
     if (t4 == 0) {
@@ -264,11 +303,10 @@ __global__ void __launch_bounds__(kThreads) prefix_decode_kernel(const __grid_co
   }
   __syncthreads();
   if (ncl > 1) cluster.sync();  // every CTA of the cluster runs: rank 0's memory may be written
-  float* dst = ncl > 1 ? cluster.map_shared_rank(gathered, 0) : gathered;
   for (int t = tid; t < G * D; t += kThreads) {
     const int hd = t / D, d = t % D;
     const float* w = reinterpret_cast<const float*>(smem) + hd * PART;
-    constexpr int WS = STAGES * 2 * TILE / 4;
+    constexpr int WS = WRING / 4;
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) mx = fmaxf(mx, w[i * WS]);
@@ -279,7 +317,8 @@ __global__ void __launch_bounds__(kThreads) prefix_decode_kernel(const __grid_co
       ls += w[i * WS + 1] * f;
       as += w[i * WS + 2 + d] * f;
     }
-    float* o = dst + (rank * G + hd) * PART;
+    float* o = gathered(rank, hd);
+    if (ncl > 1) o = cluster.map_shared_rank(o, 0);
     o[2 + d] = as;
     if (d == 0) {
       o[0] = mx;
@@ -287,25 +326,49 @@ __global__ void __launch_bounds__(kThreads) prefix_decode_kernel(const __grid_co
     }
   }
   if (ncl > 1) cluster.sync(); else __syncthreads();
+  // The rows above streamed in while the prefix launch ran; its partials (and the
+  // memory written below) only now.  Every block waits, so this launch ends after it.
+  griddep_wait();
   if (rank == 0) {
+    // factor of every partial (the prefix's, then the cluster's), and 1 / sum
+    const int64_t row = (int64_t)b * p.hq + h * G, nrows = (int64_t)p.batch * p.hq;
+    const int np_ = p.parts, all = np_ + ncl;
+    float* fac = reinterpret_cast<float*>(smem);  // [G][all], in the first slot
+    for (int hd = warp; hd < G; hd += kWarps) {
+      float mx = -INFINITY, ls = 0.f;
+      auto ml = [&](int i) {
+        return i < np_ ? *reinterpret_cast<const float2*>(p.ml + (i * nrows + row + hd) * 2)
+                       : *reinterpret_cast<const float2*>(gathered(i - np_, hd));
+      };
+      for (int i = lane; i < all; i += 32) mx = fmaxf(mx, ml(i).x);
+      for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      for (int i = lane; i < all; i += 32) {
+        const float2 v = ml(i);
+        const float f = merge_weight(v.x, mx);
+        fac[hd * all + i] = f;
+        ls += v.y * f;
+      }
+      for (int x = 16; x > 0; x >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, x);
+      const float inv = ls == 0.f ? 0.f : 1.f / ls;
+      __syncwarp();
+      for (int i = lane; i < all; i += 32) fac[hd * all + i] *= inv;
+      if (p.scores != nullptr && lane < ncl) {
+        float* st = ncl > 1 ? cluster.map_shared_rank(stat, lane) : stat;
+        st[2 * hd] = mx == -INFINITY ? 0.f : mx;
+        st[2 * hd + 1] = inv;
+      }
+    }
+    __syncthreads();
     for (int t = tid; t < G * D; t += kThreads) {
       const int hd = t / D, d = t % D;
-      float mx = -INFINITY;
-      for (int r = 0; r < ncl; ++r) mx = fmaxf(mx, gathered[(r * G + hd) * PART]);
-      float ls = 0.f, as = 0.f;
-      for (int r = 0; r < ncl; ++r) {
-        const float* o = gathered + (r * G + hd) * PART;
-        const float f = merge_weight(o[0], mx);
-        ls += o[1] * f;
-        as += o[2 + d] * f;
-      }
-      static_cast<T*>(p.out)[b * p.ob + (int64_t)(h * G + hd) * p.oh + d] = Elem<T>::from_f(ls == 0.f ? 0.f : as / ls);
-      if (d == 0 && p.scores != nullptr)
-        for (int r = 0; r < ncl; ++r) {
-          float* st = ncl > 1 ? cluster.map_shared_rank(stat, r) : stat;
-          st[2 * hd] = mx == -INFINITY ? 0.f : mx;
-          st[2 * hd + 1] = ls == 0.f ? 0.f : 1.f / ls;
-        }
+      float as = 0.f;
+      const float* pa = p.acc + (row + hd) * D + d;
+#pragma unroll 8
+      for (int i = 0; i < np_; ++i) as = fmaf(pa[i * nrows * D], fac[hd * all + i], as);
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < ncl) as = fmaf(gathered(r, hd)[2 + d], fac[hd * all + np_ + r], as);
+      static_cast<T*>(p.out)[b * p.ob + (int64_t)(h * G + hd) * p.oh + d] = Elem<T>::from_f(as);
     }
   }
   if (p.scores == nullptr) return;
@@ -326,7 +389,7 @@ template <typename T, int D, int KEYS, int STAGES>
 int launch_decode(DecodeParams& p, int ncl, cudaStream_t s) {
   auto kern = prefix_decode_kernel<T, D, KEYS, STAGES>;
   const size_t smem = kRingBytes<D, KEYS, STAGES> +
-                      4 * ((size_t)ncl * p.group * (D + 2) + 2 * p.group + (size_t)p.group * p.logit_rows);
+                      4 * (2 * p.group + (size_t)p.group * p.logit_rows);
   const cudaError_t a = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (a != cudaSuccess) return (int)a;
   cudaLaunchConfig_t cfg = {};
@@ -334,29 +397,48 @@ int launch_decode(DecodeParams& p, int ncl, cudaStream_t s) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)ncl;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.parts ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   note_launch();
   return e == cudaSuccess ? KANI_OK : (int)e;
 }
 
-// CTAs per (stream, KV head): as many as still fit the GPU at two per SM
-int cluster_size(int64_t batch, int32_t hk) {
-  int ncl = 8;
-  while (ncl > 1 && batch * hk * ncl > 2 * sm_count()) ncl >>= 1;
-  return ncl;
-}
+struct DecodePlan {
+  int ncl;         // CTAs per (stream, KV head)
+  int logit_rows;  // rows of logits that a CTA keeps in shared memory; 0: in the workspace
+  int parts;       // partial results of the prefix per query; 0: no launch for it
+  prefix::FlashSplit split;
+  int64_t logits, acc, ml;  // bytes of the workspace's sections
+};
 
-// rows of logits that a CTA keeps in shared memory; 0: they go to the workspace
-int logit_rows(int group, int64_t cache_len, int ncl) {
-  const int64_t rows = (cache_len + ncl - 1) / ncl;
-  return rows * group * 4 <= kLogitSmem ? (int)rows : 0;
+DecodePlan plan_decode(int64_t batch, int hq, int hk, int d, int64_t cache_len, int64_t prefix_rows, bool scores) {
+  DecodePlan p = {};
+  // as many CTAs as still fit the GPU at two per SM
+  p.ncl = 8;
+  while (p.ncl > 1 && batch * hk * p.ncl > 2 * sm_count()) p.ncl >>= 1;
+  const int64_t rows = (cache_len + p.ncl - 1) / p.ncl;
+  if (scores && rows * (hq / hk) * 4 <= kLogitSmem) p.logit_rows = (int)rows;
+  if (scores && !p.logit_rows) p.logits = batch * hq * cache_len * 4;
+  // The prefix in a launch of its own, for all streams, costs 3-6 us; read by every
+  // stream's blocks it costs L2 bandwidth in the streams' number.  Measured (8 KV heads
+  // of 64, up to 500 own rows; own launch / read by each): 16 streams x 1024 rows
+  // (64 MB in all) 13.2 / 10.4 us, 64 x 1024 (256 MB) 19.0 / 34 us, 16 x 4096 (256 MB)
+  // 16.1 / 23.3 us, 64 x 256 (64 MB) 21.6 / 17.9 us.
+  if (prefix_rows > 0 && batch * prefix_rows * hk * d * 4 >= kSharedBytes) {
+    p.split = prefix::flash_split(1, batch, hq, hk, prefix_rows, kMaxParts);
+    p.parts = p.split.parts;
+    p.acc = (int64_t)p.parts * batch * hq * d * 4;
+    p.ml = (int64_t)p.parts * batch * hq * 2 * 4;
+  }
+  return p;
 }
 
 }  // namespace
@@ -365,10 +447,12 @@ int logit_rows(int group, int64_t cache_len, int ncl) {
 extern "C" int64_t kani_prefix_decode_workspace(int64_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                                 int32_t head_dim, int64_t cache_len, int64_t prefix_rows,
                                                 int32_t with_scores) {
-  using namespace kani;
-  if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || cache_len <= 0 || !with_scores) return 0;
-  if (logit_rows(num_q_heads / num_kv_heads, cache_len, cluster_size(batch, num_kv_heads)) > 0) return 0;
-  return batch * num_q_heads * cache_len * 4;
+  if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || cache_len < 0 || prefix_rows < 0 ||
+      num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > 8)
+    return 0;
+  const kani::DecodePlan p =
+      kani::plan_decode(batch, num_q_heads, num_kv_heads, head_dim, cache_len, prefix_rows, with_scores && cache_len > 0);
+  return p.logits + p.acc + p.ml;
 }
 
 extern "C" int kani_prefix_decode_attention(
@@ -409,15 +493,33 @@ extern "C" int kani_prefix_decode_attention(
   p.oh = out_head_stride;
   p.err = err_flag;
   if (const int bad = prefix::check_params(p, dtype, batch, 1, num_q_heads, num_kv_heads, head_dim, scale)) return bad;
-  const int64_t need = kani_prefix_decode_workspace(batch, num_q_heads, num_kv_heads, head_dim, cache_len, prefix_rows,
-                                                    p.scores != nullptr);
+  const DecodePlan plan =
+      plan_decode(batch, num_q_heads, num_kv_heads, head_dim, cache_len, prefix_rows, p.scores != nullptr);
+  const int64_t need = plan.logits + plan.acc + plan.ml;
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace)))) return KANI_ERR_INVALID_ARG;
-  const int ncl = cluster_size(batch, num_kv_heads);
-  p.logit_rows = p.scores ? logit_rows(p.group, cache_len, ncl) : 0;
-  p.logits = p.scores && !p.logit_rows ? static_cast<float*>(workspace) : nullptr;
+  char* ws = static_cast<char*>(workspace);
+  float* acc = reinterpret_cast<float*>(ws);
+  float* ml = reinterpret_cast<float*>(ws + plan.acc);
+  p.acc = acc;
+  p.ml = ml;
+  p.parts = plan.parts;
+  // Finding a block's place costs it up to 0.4 us: worth it while the blocks make few
+  // waves (64 streams x 8 heads), not for more (128 x 8, 20 rows each: 24.1 us without
+  // it, 26.8 with).
+  p.by_length = batch > 1 && batch <= kThreads && batch * num_kv_heads * plan.ncl <= 4 * sm_count();
+  p.logit_rows = plan.logit_rows;
+  p.logits = plan.logits ? reinterpret_cast<float*>(ws + plan.acc + plan.ml) : nullptr;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (plan.parts) {  // the prefix for all streams at once: the streams are the tokens of one sequence
+    prefix::Params f = p;
+    f.qt = p.qb;
+    f.qb = 0;
+    const int rc = prefix::launch_flash(f, dtype, head_dim, 1, (int)batch, false, plan.split, ml, acc, s);
+    if (rc != KANI_OK) return rc;
+  }
   auto go = [&]<typename T>() {
-    return head_dim == 64 ? launch_decode<T, 64, 32, 3>(p, ncl, s) : launch_decode<T, 128, 16, 3>(p, ncl, s);
+    // rings of 64 KB (three blocks per SM); deeper or finer ones measured up to 20 % slower
+    return head_dim == 64 ? launch_decode<T, 64, 32, 2>(p, plan.ncl, s) : launch_decode<T, 128, 16, 2>(p, plan.ncl, s);
   };
   return dtype == KANI_DTYPE_BF16 ? go.template operator()<__nv_bfloat16>() : go.template operator()<__half>();
 }

@@ -7,15 +7,20 @@
 namespace kani {
 namespace prefix {
 
-// Splits of `rows` K / V rows over CTAs, for batch x tokens x hq query rows.
-int flash_splits(int64_t batch, int64_t tokens, int hq, int hk, int64_t rows);
+// How the K / V rows of each 128 queries of a KV head are split over CTAs: `parts`
+// clusters of `cluster` CTAs, whose results the cluster joins.
+struct FlashSplit {
+  int cluster, parts;
+};
+FlashSplit flash_split(int64_t batch, int64_t tokens, int hq, int hk, int64_t rows, int most_parts);
 
 // One launch.  own_rows: with the streams' own rows (the prompt pass), else the prefix
-// alone, of all of batch x tokens queries.  ml / acc: partials [splits][rows][2] and
-// [splits][rows][D] (fp32; maximum in powers of 2, sum, unnormalised output; a sum of
-// 0 = no row seen); NULL (one split only): the result goes to p.out.
-int launch_flash(const Params& p, int32_t dtype, int d, int batch, int tokens, bool own_rows, int splits, float* ml,
-                 float* acc, bool dependent, cudaStream_t s);
+// alone, of all of batch x tokens queries.  ml / acc: partials [parts][rows][2] and
+// [parts][rows][D] (fp32; maximum in powers of 2, sum, unnormalised output; a sum of
+// 0 = no row seen, with an output of zeros); NULL (one part only): the result goes to
+// p.out.
+int launch_flash(const Params& p, int32_t dtype, int d, int batch, int tokens, bool own_rows, FlashSplit split,
+                 float* ml, float* acc, cudaStream_t s);
 
 }  // namespace prefix
 }  // namespace kani

@@ -27,13 +27,18 @@
 // finite (0 * inf would reach every row); values that are not finite and that later
 // queries of the tile do see are added to those at the end.
 //
-// A grid of few CTAs splits the rows over several (partial maximum, sum and O in the
-// workspace) and a second kernel joins them in order.
+// A grid of few CTAs splits the rows over a cluster of 2, 4 or 8: every CTA leaves its
+// O in its own (by then idle) operand memory, and CTA r joins rows [128 r / n, ..) of
+// all of them through distributed shared memory, in the order of the splits.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "prefix_attn.cuh"
 #include "prefix_flash.cuh"
 #include "tc_common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace kani {
 namespace prefix {
@@ -53,6 +58,7 @@ template <int D> struct FlashShape {
   static constexpr uint32_t kQBytes = kRows * D * 2;
   static constexpr uint32_t kTileBytes = kKeys * D * 2;
   // 2 CTAs per SM by shared memory, so two blocks' 256 columns fill tensor memory
+  static_assert((size_t)kRows * (D + 4) * 4 <= kQBytes + (size_t)kStages * 2 * kTileBytes, "O fits the operands' memory");
   static constexpr size_t kSmem = 1024 + kQBytes + (size_t)kStages * 2 * kTileBytes;
 };
 
@@ -65,12 +71,12 @@ struct FlashParams {
   int64_t vb, vh, vs;  // strides of the own V rows (elements)
   void* out;
   int64_t ob, ot, oh;
-  float* ml;   // partials [splits][rows][2]; NULL: write out
-  float* acc;  // [splits][rows][D]
+  float* ml;   // partials [splits / cluster][rows][2]; NULL: write out
+  float* acc;  // [splits / cluster][rows][D]
   int64_t rows;  // batch * tokens * hq
   int32_t* err;
   float qscale;
-  int tokens, group, hq, tpt, splits, m_tiles;
+  int tokens, group, hq, tpt, splits, cluster, m_tiles;
   int prefix_rows, cache_len;  // cache_len 0: prefix only
   int b_step, h_step;          // 0 where the own caches' batch / head dimension is expanded
   int ph_step, qb_step;
@@ -172,6 +178,8 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
   __shared__ __align__(8) FlashBars bars;
   __shared__ uint32_t s_tmem;
   __shared__ int s_failed, s_poison;
+  __shared__ float2 s_ml[kRows];  // with a cluster: this CTA's maximum and sum of each row
+  constexpr int RED = D + 4;      // floats per row of O left in shared memory (16-byte steps between rows)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = (int)blockIdx.x % p.splits;
@@ -182,6 +190,7 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
   const uint32_t q_smem = base, ring = base + Shape::kQBytes;
 
   if (warp == 5) tc::tmem_alloc(&s_tmem, kTmemCols);
+  if (warp == 4 && lane < 5) tc::prefetch_map(lane == 0 ? &p.q : lane == 1 ? &p.pk : lane == 2 ? &p.pv : lane == 3 ? &p.k : &p.v);
   if (tid == 0) {
     s_failed = 0;
     s_poison = 0;
@@ -223,6 +232,19 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
   tc::fence_after_sync();
   const uint32_t tmem = s_tmem;
 
+  // n finished (or, for partials, unnormalised) columns from c on of the tile's row r
+  auto store = [&](int r, int c, float2 ml, const float* f, int n) {
+    const int tok = t0 + r / G, hq = h * G + r % G;
+    if (p.ml) {
+      const int64_t at = (int64_t)(split / p.cluster) * p.rows + ((int64_t)b * p.tokens + tok) * p.hq + hq;
+      if (c == 0) *reinterpret_cast<float2*>(p.ml + at * 2) = ml;
+      for (int i = 0; i < n; i += 4)
+        *reinterpret_cast<float4*>(p.acc + at * D + c + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+    } else {
+      T* o = static_cast<T*>(p.out) + b * p.ob + (int64_t)tok * p.ot + (int64_t)hq * p.oh + c;
+      for (int i = 0; i < n; i += 8) st16(o + i, pack16<T>(f + i));
+    }
+  };
   auto stage_k = [&](int j) { return ring + (uint32_t)(j % ST) * 2u * Shape::kTileBytes; };
   auto bar = [&](const uint64_t& x) { return tc::smem_addr(&x); };
 
@@ -392,15 +414,10 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
     tc::fence_after_sync();
     asm volatile("bar.sync 1, 128;" ::: "memory");  // every warp's s_poison
     const int poisoned = *(volatile int*)&s_poison;
-    const float inv = p.ml ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-    const int hq = h * G + tid % G;
-    const int64_t row = ((int64_t)b * p.tokens + tok) * p.hq + hq;
-    T* o = static_cast<T*>(p.out) + b * p.ob + (int64_t)tok * p.ot + (int64_t)hq * p.oh;
-    float* pa = p.acc + ((int64_t)split * p.rows + row) * D;
-    if (p.ml && row_ok) {
-      p.ml[((int64_t)split * p.rows + row) * 2] = m;
-      p.ml[((int64_t)split * p.rows + row) * 2 + 1] = ok && real ? l : 0.f;  // 0: nothing seen
-    }
+    const bool seen = ok && nt > 0 && real && l != 0.f;
+    const float inv = p.ml || p.cluster > 1 ? 1.f : (seen ? 1.f / l : 0.f);
+    float* red = reinterpret_cast<float*>(smem_raw + (base - tc::smem_addr(smem_raw))) + tid * RED;
+    if (p.cluster > 1) s_ml[tid] = make_float2(m, seen ? l : 0.f);
 #pragma unroll 1
     for (int c = 0; c < D; c += 32) {
       float f[32];
@@ -409,7 +426,7 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
         tmem_ld32(lanes + kTmemO + (uint32_t)c, raw);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = l == 0.f ? 0.f : __uint_as_float(raw[i]) * inv;
+        for (int i = 0; i < 32; ++i) f[i] = seen ? __uint_as_float(raw[i]) * inv : 0.f;
         if (poisoned) {
           // own rows of this CTA's partly visible tiles that this row does see
           const int lo = max(all / kKeys * kKeys, (max(first, np) - np) * kKeys), hi = min(lim, (first + nt - np) * kKeys);
@@ -420,54 +437,63 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
               if (r >= all && not_finite16<T>(vr[i])) f[i] += tc::from_bits16<T>(vr[i]);
           }
         }
+        if (p.cluster > 1) {  // (every operand has been read: the last product is done)
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(red + c + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) f[i] = 0.f;
       }
-      if (!row_ok) continue;
-      if (p.ml) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          *reinterpret_cast<float4*>(pa + c + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          float v8[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v8[e] = real ? f[i + e] : 0.f;
-          st16(o + c + i, pack16<T>(v8));
-        }
-      }
+      if (p.cluster == 1 && row_ok) store(tid, c, make_float2(m, seen ? l : 0.f), f, 32);
     }
   }
   tc::fence_before_sync();
   __syncthreads();
   if (warp == 5) tc::tmem_free(tmem, kTmemCols);
   if (tid == 0 && s_failed && p.err) atomicOr(p.err, KANI_FLAG_TIMEOUT);
-}
-
-// Joins the splits' partials, one warp per row, in split order.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) prefix_join_kernel(const float* ml, const float* acc, int64_t rows, int splits,
-                                                          int tokens, int hq, T* out, int64_t ob, int64_t ot,
-                                                          int64_t oh) {
-  griddep_wait();
-  constexpr int E = D / 32;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= rows) return;
-  float mx = -INFINITY;
-  for (int i = 0; i < splits; ++i) mx = fmaxf(mx, ml[(i * rows + row) * 2]);
-  float l = 0.f, a[E] = {};
-  for (int i = 0; i < splits; ++i) {
-    const float pl = ml[(i * rows + row) * 2 + 1];
-    if (pl == 0.f) continue;  // saw nothing
-    const float w = merge_weight(ml[(i * rows + row) * 2], mx);
-    l += pl * w;
-    for (int e = 0; e < E; ++e) a[e] += acc[(i * rows + row) * D + lane * E + e] * w;
+  if (p.cluster == 1) return;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();  // every CTA's O lies in its shared memory
+  const int rank = (int)cluster.block_rank(), share = kRows / p.cluster;
+  const float* red0 = reinterpret_cast<const float*>(smem_raw + (base - tc::smem_addr(smem_raw)));
+  for (int i = tid; i < share * (D / 8); i += kFlashThreads) {
+    const int r = rank * share + i / (D / 8), c = i % (D / 8) * 8;
+    if (r >= G * p.tpt || t0 + r / G >= p.tokens) continue;
+    float2 st[8];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      st[k] = k < p.cluster ? *cluster.map_shared_rank(&s_ml[r], k) : make_float2(-INFINITY, 0.f);
+      mx = fmaxf(mx, st[k].x);
+    }
+    float4 a[8], e[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      a[k] = e[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (st[k].y != 0.f) {  // else that CTA's tiles hold nothing for this row (or there is none)
+        const float* o = cluster.map_shared_rank(red0 + r * RED + c, k);
+        a[k] = *reinterpret_cast<const float4*>(o);
+        e[k] = *reinterpret_cast<const float4*>(o + 4);
+      }
+    }
+    float ls = 0.f, f[8] = {};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float w = merge_weight(st[k].x, mx);
+      ls += st[k].y * w;
+      f[0] += a[k].x * w, f[1] += a[k].y * w, f[2] += a[k].z * w, f[3] += a[k].w * w;
+      f[4] += e[k].x * w, f[5] += e[k].y * w, f[6] += e[k].z * w, f[7] += e[k].w * w;
+    }
+    if (!p.ml) {
+      const float inv = ls == 0.f ? 0.f : 1.f / ls;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = ls == 0.f ? 0.f : f[k] * inv;
+    }
+    store(r, c, make_float2(mx, ls), f, 8);
   }
-  T* o = out + row / hq / tokens * ob + row / hq % tokens * ot + row % hq * oh + lane * E;
-  for (int e = 0; e < E; ++e) o[e] = Elem<T>::from_f(l == 0.f ? 0.f : a[e] / l);
+  cluster.sync();  // the other CTAs have read this one's memory
 }
 
 // {64 elements, n1, n2, n3} map of 16-bit rows, in boxes of 64 x b1 x b2; strides in elements
@@ -488,28 +514,41 @@ int64_t m_tiles_of(int64_t tokens, int group) {
 
 }  // namespace
 
-// Splits of the rows over CTAs: enough for two CTAs per SM, each of two tiles or more.
-int flash_splits(int64_t batch, int64_t tokens, int hq, int hk, int64_t rows) {
+FlashSplit flash_split(int64_t batch, int64_t tokens, int hq, int hk, int64_t rows, int most_parts) {
   const int64_t ctas = batch * hk * m_tiles_of(tokens, hq / hk);
-  const int64_t tiles = (rows + kKeys - 1) / kKeys;
-  if (ctas >= sm_count()) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({2 * sm_count() / ctas, (tiles + 1) / 2, 64}));
+  const int64_t tiles = std::max<int64_t>(1, (rows + kKeys - 1) / kKeys);
+  FlashSplit s = {1, 1};
+  while (s.cluster < 8 && ctas * s.cluster * 2 <= 2 * sm_count() && s.cluster * 2 <= tiles) s.cluster *= 2;
+  if (s.cluster == 8)
+    s.parts = (int)std::max<int64_t>(1, std::min<int64_t>({sm_count() / (ctas * 8), tiles / 32, most_parts}));
+  return s;
 }
 
 template <typename T, int D>
-static int launch_flash_t(const FlashParams& f, int hk, int batch, bool dependent, cudaStream_t s) {
+static int launch_flash_t(const FlashParams& f, int hk, int batch, cudaStream_t s) {
   auto kern = prefix_flash_kernel<T, D>;
   const cudaError_t a =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FlashShape<D>::kSmem);
   if (a != cudaSuccess) return (int)a;
-  const cudaError_t e = launch_maybe_pdl(dependent, kern, dim3((unsigned)(f.m_tiles * f.splits), (unsigned)hk, (unsigned)batch),
-                                         dim3(kFlashThreads), FlashShape<D>::kSmem, s, f);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(f.m_tiles * f.splits), (unsigned)hk, (unsigned)batch);
+  cfg.blockDim = dim3(kFlashThreads);
+  cfg.dynamicSmemBytes = FlashShape<D>::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)f.cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, f);
   note_launch();
   return e == cudaSuccess ? KANI_OK : (int)e;
 }
 
-int launch_flash(const Params& p, int32_t dtype, int d, int batch, int tokens, bool own_rows, int splits, float* ml,
-                 float* acc, bool dependent, cudaStream_t s) {
+int launch_flash(const Params& p, int32_t dtype, int d, int batch, int tokens, bool own_rows, FlashSplit split,
+                 float* ml, float* acc, cudaStream_t s) {
   const bool bf16 = dtype == KANI_DTYPE_BF16;
   FlashParams f;
   memset(&f, 0, sizeof(f));
@@ -551,29 +590,20 @@ int launch_flash(const Params& p, int32_t dtype, int d, int batch, int tokens, b
   f.tokens = tokens;
   f.group = p.group;
   f.hq = p.hq;
-  f.splits = splits;
+  f.cluster = split.cluster;
+  f.splits = split.cluster * split.parts;
   f.m_tiles = (int)m_tiles_of(tokens, p.group);
   f.prefix_rows = (int)p.prefix_rows;
   f.cache_len = own_rows ? (int)p.cache_len : 0;
   if (bf16)
-    return d == 64 ? launch_flash_t<__nv_bfloat16, 64>(f, p.hk, batch, dependent, s)
-                   : launch_flash_t<__nv_bfloat16, 128>(f, p.hk, batch, dependent, s);
-  return d == 64 ? launch_flash_t<__half, 64>(f, p.hk, batch, dependent, s)
-                 : launch_flash_t<__half, 128>(f, p.hk, batch, dependent, s);
+    return d == 64 ? launch_flash_t<__nv_bfloat16, 64>(f, p.hk, batch, s)
+                   : launch_flash_t<__nv_bfloat16, 128>(f, p.hk, batch, s);
+  return d == 64 ? launch_flash_t<__half, 64>(f, p.hk, batch, s)
+                 : launch_flash_t<__half, 128>(f, p.hk, batch, s);
 }
 
 }  // namespace prefix
 }  // namespace kani
-
-extern "C" int64_t kani_prefix_prefill_workspace(int64_t batch, int64_t tokens, int32_t num_q_heads,
-                                                 int32_t num_kv_heads, int32_t head_dim, int64_t cache_len,
-                                                 int64_t prefix_rows) {
-  if (batch <= 0 || tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || cache_len < 0 ||
-      prefix_rows < 0 || num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > 8)
-    return 0;
-  const int n = kani::prefix::flash_splits(batch, tokens, num_q_heads, num_kv_heads, prefix_rows + cache_len);
-  return n > 1 ? (int64_t)n * batch * tokens * num_q_heads * (head_dim + 2) * 4 : 0;
-}
 
 extern "C" int kani_prefix_prefill_attention(
     int32_t dtype, int64_t batch, int64_t tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
@@ -582,10 +612,10 @@ extern "C" int kani_prefix_prefill_attention(
     int64_t cache_len, const int64_t* kv_len, const int64_t* q_len, const void* prefix_k, const void* prefix_v,
     int64_t prefix_head_stride, int64_t prefix_row_stride, int64_t prefix_rows, const int64_t* prefix_len,
     float scale, void* out, int64_t out_batch_stride, int64_t out_token_stride, int64_t out_head_stride,
-    void* workspace, int64_t workspace_bytes, int32_t* err_flag, void* stream) {
+    int32_t* err_flag, void* stream) {
   using namespace kani;
   if (batch < 0 || tokens < 0 || num_q_heads < 0 || num_kv_heads < 0 || head_dim < 0 || cache_len < 0 ||
-      prefix_rows < 0 || workspace_bytes < 0)
+      prefix_rows < 0)
     return KANI_ERR_INVALID_ARG;
   if (batch == 0 || tokens == 0 || num_q_heads == 0) return KANI_OK;
   prefix::Params p = {};
@@ -614,26 +644,7 @@ extern "C" int kani_prefix_prefill_attention(
   p.err = err_flag;
   if (const int bad = prefix::check_params(p, dtype, batch, tokens, num_q_heads, num_kv_heads, head_dim, scale))
     return bad;
-  const int64_t need = kani_prefix_prefill_workspace(batch, tokens, num_q_heads, num_kv_heads, head_dim, cache_len,
-                                                     prefix_rows);
-  if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace)))) return KANI_ERR_INVALID_ARG;
-  const int splits =
-      prefix::flash_splits(batch, tokens, num_q_heads, num_kv_heads, prefix_rows + cache_len);
-  const int64_t rows = batch * tokens * num_q_heads;
-  float* acc = splits > 1 ? static_cast<float*>(workspace) : nullptr;
-  float* ml = splits > 1 ? acc + (int64_t)splits * rows * head_dim : nullptr;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int rc = prefix::launch_flash(p, dtype, head_dim, (int)batch, (int)tokens, true, splits, ml, acc, false, s);
-  if (rc != KANI_OK || splits == 1) return rc;
-  auto join = [&]<typename T, int D>() {
-    const cudaError_t e =
-        launch_pdl(prefix::prefix_join_kernel<T, D>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s,
-                   static_cast<const float*>(ml), static_cast<const float*>(acc), rows, splits, (int)tokens,
-                   (int)num_q_heads, static_cast<T*>(out), p.ob, p.ot, p.oh);
-    note_launch();
-    return e == cudaSuccess ? (int)KANI_OK : (int)e;
-  };
-  if (dtype == KANI_DTYPE_BF16)
-    return head_dim == 64 ? join.template operator()<__nv_bfloat16, 64>() : join.template operator()<__nv_bfloat16, 128>();
-  return head_dim == 64 ? join.template operator()<__half, 64>() : join.template operator()<__half, 128>();
+  return prefix::launch_flash(p, dtype, head_dim, (int)batch, (int)tokens, true,
+                              prefix::flash_split(batch, tokens, num_q_heads, num_kv_heads, prefix_rows + cache_len, 1),
+                              nullptr, nullptr, static_cast<cudaStream_t>(stream));
 }

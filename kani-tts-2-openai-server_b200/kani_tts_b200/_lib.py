@@ -101,11 +101,10 @@ _SIGNATURES = {
                                       _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_f32,
                                       _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p],
                                      ctypes.c_int),
-    "kani_prefix_prefill_workspace": ([_c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i64, _c_i64], _c_i64),
     "kani_prefix_prefill_attention": ([_c_i32, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_i64, _c_i64, _c_i64,
                                        _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p,
                                        _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_f32,
-                                       _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p], ctypes.c_int),
+                                       _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p], ctypes.c_int),
     "kani_cache_evict": ([_c_i32, _c_i64, _c_i32, _c_i32, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64,
                           _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64,
                           _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p,

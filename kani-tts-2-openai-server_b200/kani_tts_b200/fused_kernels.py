@@ -1148,15 +1148,15 @@ def _attention_scale(scale, d: int) -> float:
 
 
 @functools.lru_cache(maxsize=1024)
-def _prefix_workspace_bytes(entry: str, device_index: int, *sizes: int) -> int:
-    return int(getattr(load_library(), entry)(*sizes))
+def _prefix_workspace_bytes(device_index: int, *sizes: int) -> int:
+    return int(load_library().kani_prefix_decode_workspace(*sizes))
 
 
-def _workspace(entry: str, dev: torch.device, *sizes: int):
+def _prefix_workspace(dev: torch.device, *sizes: int):
     """A call's device scratch.  It comes from the caching allocator on the current
     stream (inside a capture from the graph's own pool), so calls on other streams
     and other graphs never share it."""
-    n = _prefix_workspace_bytes(entry, dev.index, *sizes)
+    n = _prefix_workspace_bytes(dev.index, *sizes)
     return (torch.empty(n, dtype=torch.uint8, device=dev) if n else None), n
 
 
@@ -1216,7 +1216,7 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                                      (pv, "prefix_v")))
     flag = err_flag if err_flag is not None else error_flag(dev)
     with _launch_on(dev):
-        ws, n = _workspace("kani_prefix_decode_workspace", dev, b, hq, hk, d, s_len, rows, int(scores is not None))
+        ws, n = _prefix_workspace(dev, b, hq, hk, d, s_len, rows, int(scores is not None))
         check(lib.kani_prefix_decode_attention(
             code, b, hq, hk, d, qv.data_ptr(), qv.stride(0), qv.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
             cs[0], cs[1], cs[2], s_len, kv_len.data_ptr(), ptr(pk), ptr(pv), ph, ps, rows, ptr(plen), scale,
@@ -1272,11 +1272,10 @@ def prefix_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     flag = err_flag if err_flag is not None else error_flag(dev)
     qs = q.stride()
     with _launch_on(dev):
-        ws, n = _workspace("kani_prefix_prefill_workspace", dev, b, t, hq, hk, d, s_len, rows)
         check(lib.kani_prefix_prefill_attention(
             code, b, t, hq, hk, d, q.data_ptr(), qs[0], qs[1], qs[2], k_cache.data_ptr(), v_cache.data_ptr(),
             cs[0], cs[1], cs[2], s_len, kv_len.data_ptr(), ptr(q_len), ptr(pk), ptr(pv), ph, ps, rows, ptr(plen),
-            scale, out.data_ptr(), t * hq * d, hq * d, d, ptr(ws), n, flag.data_ptr(),
+            scale, out.data_ptr(), t * hq * d, hq * d, d, flag.data_ptr(),
             torch.cuda.current_stream(dev).cuda_stream), "kani_prefix_prefill_attention")
     return out
 

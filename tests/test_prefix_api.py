@@ -13,8 +13,8 @@ DECODE = dict(dtype=1, batch=2, hq=4, hk=2, d=64, q=A, qb=256, qh=64, k=A, v=A, 
               pv=A, ph=320, ps=64, p=5, plen=0, scale=0.125, scores=0, sb=0, sh=0, out=A, ob=256, oh=64, ws=A,
               nbytes=1 << 40, err=0, stream=0)
 PREFILL = dict(dtype=1, batch=2, t=3, hq=4, hk=2, d=64, q=A, qb=768, qt=256, qh=64, k=A, v=A, cb=1024, ch=512, cs=64,
-               s=8, n=A, ql=0, pk=A, pv=A, ph=320, ps=64, p=5, plen=0, scale=0.125, out=A, ob=768, ot=256, oh=64, ws=A,
-               nbytes=1 << 40, err=0, stream=0)
+               s=8, n=A, ql=0, pk=A, pv=A, ph=320, ps=64, p=5, plen=0, scale=0.125, out=A, ob=768, ot=256, oh=64, err=0,
+               stream=0)
 EVICT = dict(dtype=1, batch=2, hk=2, d=64, k=A, v=2 * A, cb=1024, ch=512, cs=64, s=8, sc=A, sb=16, sh=8, n=A, budget=4,
              recent=1, protect=1, ko=3 * A, vo=4 * A, cbo=512, cho=256, cso=64, so=4, sco=5 * A, sbo=8, sho=4, lo=6 * A,
              kept=0, err=0, stream=0)
