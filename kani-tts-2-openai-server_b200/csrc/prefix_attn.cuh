@@ -3,10 +3,26 @@
 // softmax's small functions.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace kani {
 namespace prefix {
+
+// Grants a kernel its most dynamic shared memory on the current device, once per
+// device (the call costs about a microsecond); 0 or a cudaError_t.
+template <typename Kernel>
+int grant_smem(Kernel kern, size_t bytes, std::atomic<uint64_t>& granted) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) dev = 63;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 63 && (granted.load(std::memory_order_relaxed) & bit)) return 0;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) return (int)e;
+  granted.fetch_or(bit, std::memory_order_relaxed);
+  return 0;
+}
 
 struct Params {
   const void* q;

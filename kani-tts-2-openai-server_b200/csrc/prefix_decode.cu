@@ -390,8 +390,8 @@ int launch_decode(DecodeParams& p, int ncl, cudaStream_t s) {
   auto kern = prefix_decode_kernel<T, D, KEYS, STAGES>;
   const size_t smem = kRingBytes<D, KEYS, STAGES> +
                       4 * (2 * p.group + (size_t)p.group * p.logit_rows);
-  const cudaError_t a = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (a != cudaSuccess) return (int)a;
+  static std::atomic<uint64_t> granted{0};
+  if (const int e = prefix::grant_smem(kern, kRingBytes<D, KEYS, STAGES> + 4 * 2 * 8 + kLogitSmem, granted)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ncl, (unsigned)p.hk, (unsigned)p.batch);
   cfg.blockDim = dim3(kThreads);

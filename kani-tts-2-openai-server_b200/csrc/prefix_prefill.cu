@@ -527,9 +527,8 @@ FlashSplit flash_split(int64_t batch, int64_t tokens, int hq, int hk, int64_t ro
 template <typename T, int D>
 static int launch_flash_t(const FlashParams& f, int hk, int batch, cudaStream_t s) {
   auto kern = prefix_flash_kernel<T, D>;
-  const cudaError_t a =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FlashShape<D>::kSmem);
-  if (a != cudaSuccess) return (int)a;
+  static std::atomic<uint64_t> granted{0};
+  if (const int e = grant_smem(kern, FlashShape<D>::kSmem, granted)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(f.m_tiles * f.splits), (unsigned)hk, (unsigned)batch);
   cfg.blockDim = dim3(kFlashThreads);

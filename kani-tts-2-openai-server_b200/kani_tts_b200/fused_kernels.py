@@ -28,7 +28,6 @@ the reference, all deliberate:
 """
 from __future__ import annotations
 
-import contextlib
 import functools
 import math
 
@@ -1066,38 +1065,52 @@ def codec_codes(tokens: torch.Tensor, eos_token: int, audio_tokens_start: int, c
     return codes, frames, status
 
 
-def _on_one_device(dev: torch.device, named) -> None:
-    """Every given tensor must be a CUDA tensor on `dev` (None is skipped)."""
+def _on_one_device(ref: torch.Tensor, what: str, named) -> int:
+    """`ref` and every given tensor (None is skipped) must be on one CUDA device; its index."""
+    require_cuda(ref, what)
+    index = ref.get_device()
     for t, w in named:
-        if t is not None:
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != index):
             require_cuda(t, w)
-            if t.device != dev:
-                raise ValueError(f"{w} is on {t.device}, q or the cache on {dev}")
+            raise ValueError(f"{w} is on {t.device}, {what} on {ref.device}")
+    return index
 
 
-def _launch_on(dev: torch.device):
-    """Makes `dev` the current device for a launch on its stream, where it is not."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _call(index: int, name: str, fn, *args) -> None:
+    """One C call on device `index`'s current stream, with that device as the current one."""
+    if torch.cuda.current_device() == index:
+        code = fn(*args, _lib.raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, _lib.raw_stream(index))
+    if code:
+        check(code, name)
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
     """Byte addresses [first, past the last) that a tensor's elements lie in."""
+    first = t.data_ptr()
+    if t.is_contiguous():
+        return first, first + t.nbytes
     if t.numel() == 0:
-        return 0, 0
+        return first, first
     last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    return first, first + (last + 1) * t.element_size()
 
 
-def _refuse_overlap(out: torch.Tensor, what: str, named) -> None:
-    """An output that a call writes while it still reads others must lie apart from them."""
-    a0, a1 = _span(out)
-    for t, w in named:
-        if t is not None:
-            b0, b1 = _span(t)
+def _refuse_overlap(outs, ins) -> None:
+    """Outputs that a call writes while it still reads its inputs must lie apart from
+    them, and may not be expanded views.  Both: (tensor or None, name) pairs."""
+    spans = [(*_span(t), w) for t, w in ins if t is not None]
+    for t, w in outs:
+        if t is None:
+            continue
+        a0, a1 = _span(t)
+        for b0, b1, other in spans:
             if a0 < b1 and b0 < a1:
-                raise ValueError(f"{what} must not overlap {w}")
-    if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
-        raise ValueError(f"{what} must not be an expanded view")
+                raise ValueError(f"{w} must not overlap {other}")
+        if 0 in t.stride() and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+            raise ValueError(f"{w} must not be an expanded view")
 
 
 def _lengths(t: torch.Tensor, n: int, what: str) -> torch.Tensor:
@@ -1152,12 +1165,20 @@ def _prefix_workspace_bytes(device_index: int, *sizes: int) -> int:
     return int(load_library().kani_prefix_decode_workspace(*sizes))
 
 
-def _prefix_workspace(dev: torch.device, *sizes: int):
+def _prefix_workspace(device: torch.device, index: int, *sizes: int):
     """A call's device scratch.  It comes from the caching allocator on the current
     stream (inside a capture from the graph's own pool), so calls on other streams
     and other graphs never share it."""
-    n = _prefix_workspace_bytes(dev.index, *sizes)
-    return (torch.empty(n, dtype=torch.uint8, device=dev) if n else None), n
+    n = _prefix_workspace_bytes(index, *sizes)
+    return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
+
+
+def _flag_ptr(err_flag: torch.Tensor | None, device: torch.device) -> int:
+    if err_flag is None:
+        return error_flag(device).data_ptr()
+    if err_flag.dtype != torch.int32 or err_flag.numel() < 1:
+        raise ValueError("err_flag must be an int32 device tensor")
+    return err_flag.data_ptr()
 
 
 def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor,
@@ -1185,43 +1206,43 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     Returns out [B, Hq, D]; zeros where a stream sees no row at all.  A length out of
     range is held to it and flagged in ``err_flag``.
     """
-    dev = q.device
-    _on_one_device(dev, ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (kv_len, "kv_len"),
-                         (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (prefix_len, "prefix_len"),
-                         (scores, "scores"), (out, "out"), (err_flag, "err_flag")))
+    index = _on_one_device(q, "q", ((k_cache, "k_cache"), (v_cache, "v_cache"), (kv_len, "kv_len"),
+                                    (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (prefix_len, "prefix_len"),
+                                    (scores, "scores"), (out, "out"), (err_flag, "err_flag")))
     lib = load_library()
     code = dtype_code(q, "q")
     (b, hk, s_len, d), cs = _own_cache(k_cache, v_cache, q)
     qv = q.squeeze(1) if q.dim() == 4 and q.shape[1] == 1 else q
     if qv.dim() != 3 or qv.shape[0] != b or qv.shape[2] != d or (qv.stride(2) != 1 and qv.numel()):
         raise ValueError(f"q must be [{b}, heads, {d}] with a contiguous last dim")
+    qb, qh, _ = qv.stride()
     hq = qv.shape[1]
     if hk == 0 or hq % hk:
         raise ValueError(f"{hq} query heads do not group over {hk} KV heads")
     kv_len = _lengths(kv_len, b, "kv_len")
     pk, pv, rows, ph, ps, plen = _shared_prefix(prefix_k, prefix_v, prefix_len, q, hk, d)
     scale = _attention_scale(scale, d)
-    sb = sh = 0
+    sb = sh = scores_at = 0
+    inputs = ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (pk, "prefix_k"), (pv, "prefix_v"),
+              (kv_len, "kv_len"))
     if scores is not None:
         if scores.dtype != torch.float32 or scores.shape != (b, hk, s_len) or (scores.stride(2) != 1 and s_len > 1):
             raise ValueError(f"scores must be fp32 [{b}, {hk}, {s_len}] with a contiguous last dim")
-        sb, sh = scores.stride()[:2]
-        _refuse_overlap(scores, "scores", ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (out, "out")))
+        sb, sh, _ = scores.stride()
+        scores_at = scores.data_ptr()
+        _refuse_overlap(((scores, "scores"),), inputs)
     if out is None:
-        out = torch.empty(b, hq, d, dtype=q.dtype, device=dev)
+        out = q.new_empty((b, hq, d))
     else:
         if out.numel() != b * hq * d or out.dtype != q.dtype or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {q.dtype} tensor of {b * hq * d} elements")
-        _refuse_overlap(out, "out", ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (pk, "prefix_k"),
-                                     (pv, "prefix_v")))
-    flag = err_flag if err_flag is not None else error_flag(dev)
-    with _launch_on(dev):
-        ws, n = _prefix_workspace(dev, b, hq, hk, d, s_len, rows, int(scores is not None))
-        check(lib.kani_prefix_decode_attention(
-            code, b, hq, hk, d, qv.data_ptr(), qv.stride(0), qv.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
-            cs[0], cs[1], cs[2], s_len, kv_len.data_ptr(), ptr(pk), ptr(pv), ph, ps, rows, ptr(plen), scale,
-            ptr(scores), sb, sh, out.data_ptr(), hq * d, d, ptr(ws), n, flag.data_ptr(),
-            torch.cuda.current_stream(dev).cuda_stream), "kani_prefix_decode_attention")
+        _refuse_overlap(((out, "out"),), inputs + ((scores, "scores"),))
+    ws, n = _prefix_workspace(q.device, index, b, hq, hk, d, s_len, rows, scores is not None)
+    _call(index, "kani_prefix_decode_attention", lib.kani_prefix_decode_attention,
+          code, b, hq, hk, d, qv.data_ptr(), qb, qh, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
+          s_len, kv_len.data_ptr(), pk.data_ptr() if rows else 0, pv.data_ptr() if rows else 0, ph, ps, rows,
+          0 if plen is None else plen.data_ptr(), scale, scores_at, sb, sh, out.data_ptr(), hq * d, d,
+          0 if ws is None else ws.data_ptr(), n, _flag_ptr(err_flag, q.device))
     return out
 
 
@@ -1246,16 +1267,15 @@ def prefix_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
             ``prefix_decode_attention``.  out: optional contiguous [B, T, Hq, D].
     Returns out [B, T, Hq, D].
     """
-    dev = q.device
-    _on_one_device(dev, ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (kv_len, "kv_len"), (q_len, "q_len"),
-                         (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (prefix_len, "prefix_len"), (out, "out"),
-                         (err_flag, "err_flag")))
+    index = _on_one_device(q, "q", ((k_cache, "k_cache"), (v_cache, "v_cache"), (kv_len, "kv_len"), (q_len, "q_len"),
+                                    (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (prefix_len, "prefix_len"),
+                                    (out, "out"), (err_flag, "err_flag")))
     lib = load_library()
     code = dtype_code(q, "q")
     (b, hk, s_len, d), cs = _own_cache(k_cache, v_cache, q)
     if q.dim() != 4 or q.shape[0] != b or q.shape[3] != d or (q.stride(3) != 1 and q.numel()):
         raise ValueError(f"q must be [{b}, tokens, heads, {d}] with a contiguous last dim")
-    t, hq = q.shape[1:3]
+    _, t, hq, _ = q.shape
     if hk == 0 or hq % hk:
         raise ValueError(f"{hq} query heads do not group over {hk} KV heads")
     kv_len = _lengths(kv_len, b, "kv_len")
@@ -1263,20 +1283,19 @@ def prefix_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     pk, pv, rows, ph, ps, plen = _shared_prefix(prefix_k, prefix_v, prefix_len, q, hk, d)
     scale = _attention_scale(scale, d)
     if out is None:
-        out = torch.empty(b, t, hq, d, dtype=q.dtype, device=dev)
+        out = q.new_empty((b, t, hq, d))
     else:
         if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)}")
-        _refuse_overlap(out, "out", ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (pk, "prefix_k"),
-                                     (pv, "prefix_v")))
-    flag = err_flag if err_flag is not None else error_flag(dev)
+        _refuse_overlap(((out, "out"),), ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (pk, "prefix_k"),
+                                          (pv, "prefix_v"), (kv_len, "kv_len"), (q_len, "q_len")))
     qs = q.stride()
-    with _launch_on(dev):
-        check(lib.kani_prefix_prefill_attention(
-            code, b, t, hq, hk, d, q.data_ptr(), qs[0], qs[1], qs[2], k_cache.data_ptr(), v_cache.data_ptr(),
-            cs[0], cs[1], cs[2], s_len, kv_len.data_ptr(), ptr(q_len), ptr(pk), ptr(pv), ph, ps, rows, ptr(plen),
-            scale, out.data_ptr(), t * hq * d, hq * d, d, flag.data_ptr(),
-            torch.cuda.current_stream(dev).cuda_stream), "kani_prefix_prefill_attention")
+    _call(index, "kani_prefix_prefill_attention", lib.kani_prefix_prefill_attention,
+          code, b, t, hq, hk, d, q.data_ptr(), qs[0], qs[1], qs[2], k_cache.data_ptr(), v_cache.data_ptr(), cs[0],
+          cs[1], cs[2], s_len, kv_len.data_ptr(), 0 if q_len is None else q_len.data_ptr(),
+          pk.data_ptr() if rows else 0, pv.data_ptr() if rows else 0, ph, ps, rows,
+          0 if plen is None else plen.data_ptr(), scale, out.data_ptr(), t * hq * d, hq * d, d,
+          _flag_ptr(err_flag, q.device))
     return out
 
 
@@ -1306,60 +1325,58 @@ def evict_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tens
     length become zero (the next rows start from there); K / V rows past it stay as
     they were.
     """
-    dev = k_cache.device
-    _on_one_device(dev, ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores"), (kv_len, "kv_len"),
-                         (k_out, "k_out"), (v_out, "v_out"), (scores_out, "scores_out"), (len_out, "len_out"),
-                         (kept_out, "kept_out"), (err_flag, "err_flag")))
+    index = _on_one_device(k_cache, "k_cache", ((v_cache, "v_cache"), (scores, "scores"), (kv_len, "kv_len"),
+                                                (k_out, "k_out"), (v_out, "v_out"), (scores_out, "scores_out"),
+                                                (len_out, "len_out"), (kept_out, "kept_out"), (err_flag, "err_flag")))
     lib = load_library()
     code = dtype_code(k_cache, "k_cache")
     (b, hk, s_len, d), cs = _own_cache(k_cache, v_cache, k_cache)
-
-    def check_scores(t, rows, what):
-        if t.dtype != torch.float32 or t.shape != (b, hk, rows) or (t.stride(2) != 1 and rows > 1):
-            raise ValueError(f"{what} must be fp32 [{b}, {hk}, {rows}] with a contiguous last dim")
-
-    check_scores(scores, s_len, "scores")
+    ss = _score_strides(scores, b, hk, s_len, "scores")
     kv_len = _lengths(kv_len, b, "kv_len")
-    given = sum(t is not None for t in (k_out, v_out, scores_out))
-    if given not in (0, 3):
+    if (k_out is None) != (v_out is None) or (k_out is None) != (scores_out is None):
         raise ValueError("k_out, v_out and scores_out must be given together (or none of them: in place)")
-    inputs = ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores"), (kv_len, "kv_len"))
-    if given:
+    inputs = ((kv_len, "kv_len"),)
+    if k_out is not None:
         (bo, hko, out_len, do), co = _own_cache(k_out, v_out, k_cache)
         if (bo, hko, do) != (b, hk, d):
             raise ValueError(f"k_out / v_out must be [{b}, {hk}, rows, {d}]")
-        check_scores(scores_out, out_len, "scores_out")
-        for t, w in ((k_out, "k_out"), (v_out, "v_out"), (scores_out, "scores_out")):
-            _refuse_overlap(t, w, inputs)
+        so = _score_strides(scores_out, b, hk, out_len, "scores_out")
+        inputs = ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores"), (kv_len, "kv_len"))
     else:
-        k_out, v_out, scores_out, out_len, co = k_cache, v_cache, scores, s_len, cs
-        for t, w in ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores")):
-            _refuse_overlap(t, w, ((kv_len, "kv_len"),))
+        k_out, v_out, scores_out, out_len, co, so = k_cache, v_cache, scores, s_len, cs, ss
     if k_out.data_ptr() == v_out.data_ptr() and k_out.numel():
         raise ValueError("keys and values must be different tensors")
     budget, recent, protect = int(budget), int(recent), int(protect)
     if budget < 0 or recent < 0 or protect < 0 or protect + recent > budget or budget > out_len:
         raise ValueError(f"0 <= protect + recent <= budget <= {out_len} expected, got protect {protect}, "
                          f"recent {recent}, budget {budget}")
-    if len_out is None:
-        len_out = torch.empty(b, dtype=torch.int64, device=dev)
-    elif len_out.dtype != torch.int64 or len_out.numel() != b or not len_out.is_contiguous():
+    if len_out is not None and (len_out.dtype != torch.int64 or len_out.numel() != b or not len_out.is_contiguous()):
         raise ValueError(f"len_out must be contiguous int64 with {b} elements")
-    else:
-        _refuse_overlap(len_out, "len_out", inputs)
+    kept_at = 0
     if kept_out is not None:
         if kept_out.dtype != torch.int32 or kept_out.shape != (b, hk, budget) or not kept_out.is_contiguous():
             raise ValueError(f"kept_out must be contiguous int32 [{b}, {hk}, {budget}]")
-        _refuse_overlap(kept_out, "kept_out", inputs)
-    flag = err_flag if err_flag is not None else error_flag(dev)
-    ss, so = scores.stride(), scores_out.stride()
-    with _launch_on(dev):
-        check(lib.kani_cache_evict(
-            code, b, hk, d, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], s_len, scores.data_ptr(),
-            ss[0], ss[1], kv_len.data_ptr(), budget, recent, protect, k_out.data_ptr(), v_out.data_ptr(), co[0],
-            co[1], co[2], out_len, scores_out.data_ptr(), so[0], so[1], len_out.data_ptr(), ptr(kept_out),
-            flag.data_ptr(), torch.cuda.current_stream(dev).cuda_stream), "kani_cache_evict")
+        kept_at = kept_out.data_ptr()
+    _refuse_overlap(((k_out, "k_out"), (v_out, "v_out"), (scores_out, "scores_out"), (len_out, "len_out"),
+                     (kept_out, "kept_out")), inputs)
+    if k_out is k_cache and (len_out is not None or kept_out is not None):
+        _refuse_overlap(((len_out, "len_out"), (kept_out, "kept_out")),
+                        ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores")))
+    if len_out is None:
+        len_out = kv_len.new_empty(b)
+    _call(index, "kani_cache_evict", lib.kani_cache_evict,
+          code, b, hk, d, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], s_len, scores.data_ptr(),
+          ss[0], ss[1], kv_len.data_ptr(), budget, recent, protect, k_out.data_ptr(), v_out.data_ptr(), co[0], co[1],
+          co[2], out_len, scores_out.data_ptr(), so[0], so[1], len_out.data_ptr(), kept_at,
+          _flag_ptr(err_flag, k_cache.device))
     return len_out
+
+
+def _score_strides(t: torch.Tensor, b: int, hk: int, rows: int, what: str):
+    st = t.stride()
+    if t.dtype != torch.float32 or t.shape != (b, hk, rows) or (st[2] != 1 and rows > 1):
+        raise ValueError(f"{what} must be fp32 [{b}, {hk}, {rows}] with a contiguous last dim")
+    return st
 
 
 def launch_count() -> int:
