@@ -9,131 +9,288 @@
 // become zero.  K / V rows past the new length stay as they were.  Streams of at
 // most `budget` rows keep all of them.
 //
-// One block per (b, h).  The lowest kept score is found by a binary search over
-// its bits; a scan over the slots then gives every kept row its destination.  In
-// place, row i comes from a slot >= i, so each step of 256 rows is read before
-// any of it is written, and no later step reads what it wrote.
+// Moving the kept rows bounds it.  A cluster of 1, 2, 4 or 8 CTAs works on one
+// (b, h): every CTA finds the kept rows for itself and moves its share of the columns
+// of the rows [K | V], so in-place moves of different CTAs never meet.
+//   * Selection: the scores' bits in an order where unsigned comparison is theirs; the
+//     most-th largest by radix selection over digits of 11, 11 and 10 bits, with a
+//     histogram in shared memory (lanes of one digit add up before the atomic: heavy
+//     ties would queue there); ties beyond it go by slot.  Counts are integers, so
+//     the order of the atomics does not matter.
+//   * Compaction: kept slots of a chunk by ballots and a scan over the warps, as a
+//     list in shared memory; then 16-byte pieces of the listed rows, four in flight
+//     per thread.  In place, kept row i comes from a slot >= i: each step's pieces are
+//     all read before any is written, and no later step reads a row that was written.
+//   * Scores stay in registers between the passes where the cache is one chunk; CTA 0
+//     writes the moved ones once every CTA of the cluster has read the chunk.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace kani {
 namespace {
 
-constexpr int kEvictThreads = 256;
+constexpr int kEvictThreads = 512;
+constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kInFlight = 4;  // 16-byte pieces per thread and step
 
 struct EvictParams {
-  const void* k;
-  const void* v;
+  const char* k;
+  const char* v;
   int64_t cb, ch, cs;  // byte strides of the caches [B, Hk, S, D]
   int64_t cache_len;
   const float* scores;
   int64_t sb, sh;
   const int64_t* kv_len;
   int64_t budget, recent, protect;
-  void* k_out;
-  void* v_out;
+  char* k_out;
+  char* v_out;
   int64_t cbo, cho, cso;
   float* scores_out;
   int64_t sbo, sho;
   int64_t out_len;
   int64_t* len_out;
   int32_t* kept;  // [B, Hk, budget] or NULL
-  int row_vecs;   // 16-byte vectors per row
+  int row_vecs;   // 16-byte pieces per row of K or V
+  int in_place;
   int32_t* err;
 };
 
 // a score's bits in an order where unsigned comparison is the score's; NaN lowest
-__device__ __forceinline__ uint32_t score_key(float f) {
-  if (isnan(f)) return 0u;
-  const uint32_t u = __float_as_uint(f + 0.f);  // -0 -> +0
+__device__ __forceinline__ uint32_t score_key(uint32_t u) {
+  if ((u & 0x7fffffffu) > 0x7f800000u) return 0u;
+  if (u == 0x80000000u) u = 0u;  // -0 is 0
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-__device__ int block_sum(int x, int* red) {
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
-  __syncthreads();
-  int s = 0;
-  for (int w = 0; w < kEvictThreads / 32; ++w) s += red[w];
-  __syncthreads();
-  return s;
-}
-
-// exclusive prefix sum of a flag over the block, and the block's total
-__device__ int block_rank(bool f, int* red, int& total) {
-  const unsigned m = __ballot_sync(0xffffffffu, f);
+// exclusive sum over the block's warps of one number per warp (given in all its
+// lanes), and the total; `red` holds kEvictWarps ints
+__device__ __forceinline__ int warps_before(int x, int* red, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (lane == 0) red[warp] = __popc(m);
+  __syncthreads();  // the last use of red is over
+  if (lane == 0) red[warp] = x;
   __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int w = 0; w < kEvictThreads / 32; ++w) {
-    if (w < warp) before += red[w];
-    total += red[w];
+  int v = lane < kEvictWarps ? red[lane] : 0, sum = v;
+#pragma unroll
+  for (int o = 1; o < kEvictWarps; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += y;
   }
-  __syncthreads();
-  return before + __popc(m & ((1u << lane) - 1u));
+  total = __shfl_sync(0xffffffffu, sum, kEvictWarps - 1);
+  return __shfl_sync(0xffffffffu, sum - v, warp);
 }
 
-__global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictParams p) {
-  __shared__ int red[kEvictThreads / 32];
-  __shared__ int s_src[kEvictThreads];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  int64_t n = p.kv_len[b];
-  if ((n < 0 || n > p.cache_len) && h == 0 && tid == 0 && p.err) atomicOr(p.err, KANI_FLAG_SLOT_OOB);
-  n = n < 0 ? 0 : (n > p.cache_len ? p.cache_len : n);
+template <int ITEMS>
+__global__ void __launch_bounds__(kEvictThreads, ITEMS > 16 ? 1 : 2) cache_evict_kernel(const EvictParams p) {
+  constexpr int CHUNK = kEvictThreads * ITEMS;  // slots per chunk; warp w has ITEMS * 32 of them in a row
+  extern __shared__ int s_list[];               // kept slots of the chunk
+  __shared__ int hist[kBins];
+  __shared__ int red[kEvictWarps];
+  __shared__ int s_digit, s_need;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ncl = (int)gridDim.x, rank = (int)blockIdx.x;
+  const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int64_t len = p.kv_len[b];
+  if ((len < 0 || len > p.cache_len) && rank == 0 && h == 0 && tid == 0 && p.err) atomicOr(p.err, KANI_FLAG_SLOT_OOB);
+  const int n = (int)(len < 0 ? 0 : (len > p.cache_len ? p.cache_len : len));
+  const bool cut = n > p.budget;
+  const int keep = cut ? (int)p.budget : n;
+  // rows [lo, hi) compete for `most` places; the others stay
+  const int lo = cut ? (int)p.protect : n, hi = cut ? n - (int)p.recent : n;
+  const int most = cut ? (int)(p.budget - p.protect - p.recent) : 0;
   const float* sc = p.scores + b * p.sb + h * p.sh;
-  const int64_t keep = n < p.budget ? n : p.budget;
-  const int64_t lo = n > p.budget ? p.protect : n, hi = n > p.budget ? n - p.recent : n;
-  const int64_t most = n > p.budget ? p.budget - p.protect - p.recent : 0;
-  // the largest threshold that at least `most` of the rows between reach
-  uint32_t thr = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t t = thr | (1u << bit);
-    int c = 0;
-    for (int64_t j = lo + tid; j < hi; j += kEvictThreads) c += score_key(sc[j]) >= t;
-    if (block_sum(c, red) >= most) thr = t;
-  }
-  int above = 0;
-  for (int64_t j = lo + tid; j < hi; j += kEvictThreads) above += score_key(sc[j]) > thr;
-  const int64_t ties = most - block_sum(above, red);  // rows at the threshold that stay
-  int64_t dst0 = 0, tie0 = 0;
-  for (int64_t j0 = 0; j0 < n; j0 += kEvictThreads) {
-    const int64_t j = j0 + tid;
-    const bool in = j < n, mid = in && j >= lo && j < hi;
-    const uint32_t key = mid ? score_key(sc[j]) : 0u;
-    int total;
-    const bool tie = mid && key == thr;
-    const int tr = block_rank(tie, red, total);
-    const bool stay = in && (!mid || key > thr || (tie && tie0 + tr < ties));
-    tie0 += total;
-    const int rank = block_rank(stay, red, total);
-    if (stay) s_src[rank] = (int)j;
-    __syncthreads();
-    const bool row = tid < total;
-    const int64_t src = row ? s_src[tid] : 0, dst = dst0 + tid;
-    for (int c = 0; c < 2 * p.row_vecs; ++c) {
-      const int vec = c >> 1;
-      const char* in_ = static_cast<const char*>(c & 1 ? p.v : p.k) + b * p.cb + h * p.ch + src * p.cs + vec * 16;
-      char* out_ = static_cast<char*>(c & 1 ? p.v_out : p.k_out) + b * p.cbo + h * p.cho + dst * p.cso + vec * 16;
-      uint4 x;
-      if (row) x = ld16(in_);
+  const int chunks = (n + CHUNK - 1) / CHUNK;
+
+  uint32_t raw[ITEMS];
+  auto slot = [&](int c, int i) { return c * CHUNK + warp * (ITEMS * 32) + i * 32 + lane; };
+  auto load = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) raw[i] = slot(c, i) < n ? __float_as_uint(sc[slot(c, i)]) : 0u;
+  };
+  if (chunks > 0) load(0);
+
+  // ---- the lowest kept score of the competing rows, and how many rows tie for it
+  uint32_t thr = 0xffffffffu;
+  int ties = 0;
+  if (most > 0) {
+    int need = most;
+    uint32_t prefix = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      for (int i = tid; i < kBins; i += kEvictThreads) hist[i] = 0;
       __syncthreads();
-      if (row) st16(out_, x);
+#pragma unroll 1
+      for (int c = 0; c < chunks; ++c) {
+        if (chunks > 1) load(c);
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+          const int j = slot(c, i);
+          const uint32_t key = score_key(raw[i]);
+          const bool in = j >= lo && j < hi && (pass == 0 || (key >> (shift + bits)) == prefix);
+          const unsigned with = __ballot_sync(0xffffffffu, in);
+          if (in) {
+            const int digit = (int)((key >> shift) & ((1u << bits) - 1u));
+            const unsigned same = __match_any_sync(with, digit);
+            if (lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+          }
+        }
+      }
+      __syncthreads();
+      // digits from the highest down: thread t has the four below 2048 - 4 t
+      const int top = kBins - 1 - 4 * tid;
+      int four[4], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += four[i] = hist[top - i];
+      int before = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += y;
+      }
+      int total;
+      const int wsum = __shfl_sync(0xffffffffu, before, 31);
+      before += warps_before(wsum, red, total) - sum;
+      if (before < need && need <= before + sum) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (need > before && need <= before + four[i]) {
+            s_digit = top - i;
+            s_need = need - before;
+          }
+          before += four[i];
+        }
+      }
+      __syncthreads();
+      prefix = (prefix << bits) | (uint32_t)s_digit;
+      need = s_need;
     }
-    const float f = row ? sc[src] : 0.f;
-    __syncthreads();
-    if (row) {
-      p.scores_out[b * p.sbo + h * p.sho + dst] = f;
-      if (p.kept) p.kept[((int64_t)b * gridDim.x + h) * p.budget + dst] = (int32_t)src;
+    thr = prefix;
+    ties = need;
+  }
+
+  // ---- the kept slots in order, chunk by chunk, and their rows
+  const int w0 = rank * 2 * p.row_vecs / ncl, wn = (rank + 1) * 2 * p.row_vecs / ncl - w0;  // pieces of [K | V]
+  const int shift = (wn & (wn - 1)) == 0 ? __ffs(wn) - 1 : -1;
+  const char* kin = p.k + b * p.cb + h * p.ch;
+  const char* vin = p.v + b * p.cb + h * p.ch;
+  char* kout = p.k_out + b * p.cbo + h * p.cho;
+  char* vout = p.v_out + b * p.cbo + h * p.cho;
+  float* so = p.scores_out + b * p.sbo + h * p.sho;
+  int32_t* kept = p.kept ? p.kept + ((int64_t)b * gridDim.y + h) * p.budget : nullptr;
+  int dst0 = 0, tie0 = 0;
+#pragma unroll 1
+  for (int c = 0; c < chunks; ++c) {
+    if (chunks > 1) load(c);
+    if (p.in_place && ncl > 1) cluster.sync();  // the chunk's scores are in every CTA's registers
+    int sure = 0, tied = 0;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int j = slot(c, i);
+      const uint32_t key = score_key(raw[i]);
+      const bool mid = j >= lo && j < hi;
+      sure += __popc(__ballot_sync(0xffffffffu, j < n && (!mid || key > thr)));
+      tied += __popc(__ballot_sync(0xffffffffu, mid && key == thr));
+    }
+    int all_tied, total;
+    int tie = tie0 + warps_before(tied, red, all_tied);  // tied rows before this warp's
+    const int stay = sure + min(max(ties - tie, 0), tied);
+    int at = warps_before(stay, red, total);  // kept rows of the chunk before this warp's
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int j = slot(c, i);
+      const uint32_t key = score_key(raw[i]);
+      const bool mid = j >= lo && j < hi, tied_row = mid && key == thr;
+      const unsigned below = (1u << lane) - 1u, tm = __ballot_sync(0xffffffffu, tied_row);
+      const bool stays = j < n && (!mid || key > thr || (tied_row && tie + __popc(tm & below) < ties));
+      const unsigned sm = __ballot_sync(0xffffffffu, stays);
+      if (stays) {
+        const int r = at + __popc(sm & below);
+        s_list[r] = j;
+        if (rank == 0) {
+          so[dst0 + r] = __uint_as_float(raw[i]);
+          if (kept) kept[dst0 + r] = j;
+        }
+      }
+      tie += __popc(tm);
+      at += __popc(sm);
+    }
+    __syncthreads();  // the list is complete
+
+    // pieces: index = row * wn + piece
+    const int64_t pieces = (int64_t)total * wn;
+    auto where = [&](int64_t i, int& r, int& w) {
+      if (shift >= 0) {
+        r = (int)(i >> shift);
+        w = w0 + (int)(i & (wn - 1));
+      } else {
+        r = (int)(i / wn);
+        w = w0 + (int)(i % wn);
+      }
+    };
+    for (int64_t i0 = 0; i0 < pieces; i0 += kEvictThreads * kInFlight) {
+      uint4 x[kInFlight];
+      char* to[kInFlight];
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u) {
+        const int64_t i = i0 + u * kEvictThreads + tid;
+        to[u] = nullptr;
+        if (i < pieces) {
+          int r, w;
+          where(i, r, w);
+          const int src = s_list[r], dst = dst0 + r;
+          if (!p.in_place || src != dst) {
+            const bool val = w >= p.row_vecs;
+            const int64_t off = (int64_t)(val ? w - p.row_vecs : w) * 16;
+            x[u] = ld16_stream((val ? vin : kin) + src * p.cs + off);
+            to[u] = (val ? vout : kout) + dst * p.cso + off;
+          }
+        }
+      }
+      if (p.in_place) __syncthreads();  // every piece of this step is in registers
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+        if (to[u] != nullptr) st16(to[u], x[u]);
     }
     dst0 += total;
-    __syncthreads();
+    tie0 += all_tied;
+    if (c + 1 < chunks) __syncthreads();  // the list may be overwritten
   }
-  for (int64_t j = keep + tid; j < p.out_len; j += kEvictThreads) p.scores_out[b * p.sbo + h * p.sho + j] = 0.f;
-  if (p.kept)
-    for (int64_t j = keep + tid; j < p.budget; j += kEvictThreads)
-      p.kept[((int64_t)b * gridDim.x + h) * p.budget + j] = -1;
-  if (h == 0 && tid == 0) p.len_out[b] = keep;
+  if (p.in_place && ncl > 1 && chunks == 0) cluster.sync();
+  if (rank == 0) {
+    for (int64_t j = keep + tid; j < p.out_len; j += kEvictThreads) so[j] = 0.f;
+    if (kept)
+      for (int64_t j = keep + tid; j < p.budget; j += kEvictThreads) kept[j] = -1;
+    if (h == 0 && tid == 0) p.len_out[b] = keep;
+  }
+}
+
+template <int ITEMS>
+int launch_evict(const EvictParams& p, int ncl, int hk, int batch, cudaStream_t s) {
+  auto kern = cache_evict_kernel<ITEMS>;
+  const size_t smem = (size_t)kEvictThreads * ITEMS * sizeof(int);
+  if (smem > 32 * 1024) {
+    const cudaError_t a = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (a != cudaSuccess) return (int)a;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ncl, (unsigned)hk, (unsigned)batch);
+  cfg.blockDim = dim3(kEvictThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ncl;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  note_launch();
+  return e == cudaSuccess ? KANI_OK : (int)e;
 }
 
 }  // namespace
@@ -155,28 +312,33 @@ extern "C" int kani_cache_evict(int32_t dtype, int64_t batch, int32_t num_kv_hea
   if (dtype != KANI_DTYPE_F32 && dtype != KANI_DTYPE_BF16 && dtype != KANI_DTYPE_F16) return KANI_ERR_DTYPE;
   if (batch == 0 || num_kv_heads == 0) return KANI_OK;
   const int es = dtype == KANI_DTYPE_F32 ? 4 : 2;
-  const bool rows = cache_len > 0 && out_len > 0 && head_dim > 0;
-  if (!kv_len || !len_out || kv_len == len_out ||
-      (rows && (!k_cache || !v_cache || !k_out || !v_out || !scores || !scores_out || k_cache == v_cache || k_out == v_out)))
+  if (head_dim == 0 || !kv_len || !len_out || kv_len == len_out ||
+      (cache_len > 0 && (!k_cache || !v_cache || !scores || k_cache == v_cache)) ||
+      (out_len > 0 && (!k_out || !v_out || !scores_out || k_out == v_out)))
     return KANI_ERR_INVALID_ARG;
   // in place is all of k, v and scores in place
-  const bool in_place = rows && k_out == k_cache;
-  if (rows && ((v_out == v_cache) != in_place || (scores_out == scores) != in_place)) return KANI_ERR_INVALID_ARG;
+  const bool in_place = cache_len > 0 && k_out == k_cache;
+  if (cache_len > 0 && ((v_out == v_cache) != in_place || (scores_out == scores) != in_place))
+    return KANI_ERR_INVALID_ARG;
   if (in_place && (out_batch_stride != cache_batch_stride || out_head_stride != cache_head_stride ||
                    out_slot_stride != cache_slot_stride || out_len != cache_len ||
                    scores_out_batch_stride != scores_batch_stride || scores_out_head_stride != scores_head_stride))
     return KANI_ERR_INVALID_ARG;
-  const int64_t st[] = {cache_batch_stride, cache_head_stride, cache_slot_stride,
-                        out_batch_stride,   out_head_stride,   out_slot_stride};
-  for (int64_t x : st)
+  // the strides of dimensions of one element are never followed
+  if (batch == 1) cache_batch_stride = out_batch_stride = 0;
+  if (num_kv_heads == 1) cache_head_stride = out_head_stride = 0;
+  if (cache_len <= 1) cache_slot_stride = 0;
+  if (out_len <= 1) out_slot_stride = 0;
+  for (int64_t x : {cache_batch_stride, cache_head_stride, cache_slot_stride, out_batch_stride, out_head_stride,
+                    out_slot_stride})
     if (x * es % 16 != 0) return KANI_ERR_UNSUPPORTED;
   if ((int64_t)head_dim * es % 16 != 0 || head_dim > 256 || batch > 65535 || num_kv_heads > 65535 ||
       cache_len > (1 << 30) || out_len > (1 << 30) || !aligned16(k_cache) || !aligned16(v_cache) ||
       !aligned16(k_out) || !aligned16(v_out))
     return KANI_ERR_UNSUPPORTED;
   EvictParams p = {};
-  p.k = k_cache;
-  p.v = v_cache;
+  p.k = static_cast<const char*>(k_cache);
+  p.v = static_cast<const char*>(v_cache);
   p.cb = cache_batch_stride * es;
   p.ch = cache_head_stride * es;
   p.cs = cache_slot_stride * es;
@@ -188,8 +350,8 @@ extern "C" int kani_cache_evict(int32_t dtype, int64_t batch, int32_t num_kv_hea
   p.budget = budget;
   p.recent = recent;
   p.protect = protect;
-  p.k_out = k_out;
-  p.v_out = v_out;
+  p.k_out = static_cast<char*>(k_out);
+  p.v_out = static_cast<char*>(v_out);
   p.cbo = out_batch_stride * es;
   p.cho = out_head_stride * es;
   p.cso = out_slot_stride * es;
@@ -201,7 +363,13 @@ extern "C" int kani_cache_evict(int32_t dtype, int64_t batch, int32_t num_kv_hea
   p.kept = kept_out;
   p.row_vecs = head_dim * es / 16;
   p.err = err_flag;
-  cache_evict_kernel<<<dim3((unsigned)num_kv_heads, (unsigned)batch), kEvictThreads, 0,
-                       static_cast<cudaStream_t>(stream)>>>(p);
-  return launch_status();
+  p.in_place = in_place;
+  // enough CTAs for two per SM, each with 32 bytes or more of a row
+  int ncl = 1;
+  while (ncl < 8 && batch * num_kv_heads * ncl * 2 <= 2 * sm_count() && ncl * 2 <= p.row_vecs) ncl *= 2;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // one chunk where the cache allows it, of few slots where it is short
+  if (cache_len <= kEvictThreads * 4) return launch_evict<4>(p, ncl, num_kv_heads, (int)batch, s);
+  if (cache_len <= kEvictThreads * 16) return launch_evict<16>(p, ncl, num_kv_heads, (int)batch, s);
+  return launch_evict<32>(p, ncl, num_kv_heads, (int)batch, s);
 }
