@@ -18,9 +18,9 @@
 //   * warps 0..3 hold one query row per thread: maximum, p = 2^(s c - m), sum in
 //     fp32; P is rounded to the storage type (bf16 / fp16: half a step of it relative
 //     to each weight, as the result's own rounding) and replaces S in tensor memory.
-// The running maximum moves only when a logit passes it by 2^8, so O is rescaled
-// (read from and written back to tensor memory) a few times per row at most; p stays
-// below 2^8, which both types hold.
+// The running maximum moves only when a tile's weights sum to more than 2^10, so most
+// tiles need no search for it, and O is rescaled (read from and written back to tensor
+// memory) a few times per row at most; p stays below 2^10, which both types hold.
 //
 // Rows that a tile holds beyond what its queries may see are masked in S, and their
 // V is replaced by zeros in shared memory where nobody may see it or where it is not
@@ -50,11 +50,16 @@ constexpr int kSoftmaxThreads = 128;
 constexpr int kFlashThreads = kSoftmaxThreads + 64;
 constexpr uint32_t kTmemCols = 256;  // S: 2 x 64, O: D
 constexpr uint32_t kTmemO = 128;
-constexpr float kMaxSlack = 8.f;
+constexpr float kMaxSum = 1024.f;
 constexpr int kMaxStages = 4;
 
 template <int D> struct FlashShape {
   static constexpr int kStages = D == 64 ? 4 : 2;
+  // One pair of weights in so many by polynomial instead of the special-function unit,
+  // which takes 8 cycles for a warp's 32: with D = 64 that unit bounds the kernel (4 x
+  // 4096 tokens behind 4096 rows: none 610 us, one in 4 552, one in 3 555), with D = 128
+  // the products weigh twice as much (3 x 777 tokens: none 55.7 us, one in 4 58.0).
+  static constexpr int kFmaOneIn = D == 64 ? 4 : 0;
   static constexpr uint32_t kQBytes = kRows * D * 2;
   static constexpr uint32_t kTileBytes = kKeys * D * 2;
   // 2 CTAs per SM by shared memory, so two blocks' 256 columns fill tensor memory
@@ -164,6 +169,39 @@ __device__ __forceinline__ bool not_finite16(uint32_t bits) {
   return (bits & e) == e;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x on the FMA pipes, for x < 128: x = n + f with n the nearest integer (read off the
+// low bits of x + 1.5 * 2^23), 2^f by a polynomial of degree 4 fitted to the least
+// relative error on [-1/2, 1/2] (2.7e-6, under a hundredth of half a step of fp16), n
+// added to the exponent.  Below 2^-126 it stays there.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 magic = make_float2(12582912.f, 12582912.f);
+  const float2 t = __fadd2_rn(x, magic);
+  const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = __fadd2_rn(x, make_float2(-n.x, -n.y));
+  auto k = [](float v) { return make_float2(v, v); };
+  float2 p = __ffma2_rn(k(0.009570102207362652f), f, k(0.05591785907745361f));
+  p = __ffma2_rn(p, f, k(0.240247443318367f));
+  p = __ffma2_rn(p, f, k(0.6931217908859253f));
+  p = __ffma2_rn(p, f, k(0.9999992847442627f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
+// one lane of a converged warp (which the compiler knows to be one)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+  return ok != 0;
+}
+
 struct FlashBars {
   uint64_t q, pv;
   uint64_t kv_full[kMaxStages], kv_empty[kMaxStages];
@@ -249,7 +287,7 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
   auto bar = [&](const uint64_t& x) { return tc::smem_addr(&x); };
 
   if (warp == 4) {
-    if (lane == 0 && nt > 0) {
+    if (nt > 0 && elect_one()) {
       tc::expect_tx(bar(bars.q), (uint32_t)(G * p.tpt) * D * 2);
 #pragma unroll
       for (int c = 0; c < D / 64; ++c)
@@ -279,7 +317,7 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
       if (!ok) atomicOr(&s_failed, 1);
     }
   } else if (warp == 5) {
-    if (lane == 0 && nt > 0) {
+    if (nt > 0 && elect_one()) {
       const uint32_t id_s = tc::idesc_f16<T>(kRows, kKeys);
       const uint32_t id_o = tc::idesc_f16<T>(kRows, D) | (1u << 16);  // B is MN-major
       auto qk = [&](int j) {
@@ -328,26 +366,59 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
       if (!wait_all(bars.s_full[j & 1], (uint32_t)((j >> 1) & 1))) break;
       tc::fence_after_sync();
       const uint32_t sp = lanes + (uint32_t)(j & 1) * 64u;
-      uint32_t s[64];
-      tmem_ld32(sp, s);
-      tmem_ld32(sp + 32u, s + 32);
-      tmem_wait_ld();
       const int jt = first + j;
       const bool pre = jt < np;
       const int row0 = (pre ? jt : jt - np) * kKeys;
       const bool ragged = row0 + kKeys > (pre ? plen : all);  // some row may not see all of the tile
-      if (ragged) {
-        const int n = (pre ? (real ? plen : 0) : lim) - row0;
+      const int n = ragged ? (pre ? (real ? plen : 0) : lim) - row0 : kKeys;  // of them this row sees the first n
+      auto load_s = [&](uint32_t (&s)[64]) {
+        tmem_ld32(sp, s);
+        tmem_ld32(sp + 32u, s + 32);
+        tmem_wait_ld();
+        if (ragged) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (i >= n) s[i] = 0xff800000u;  // -inf
+          for (int i = 0; i < 64; ++i)
+            if (i >= n) s[i] = 0xff800000u;  // -inf
+        }
+      };
+      // The weights relative to the maximum so far, without looking for a new one: a
+      // sum that passes 2^10 (or a first look at the row) shows that it is needed.
+      uint32_t pk[32];
+      float tile_sum = 0.f;
+      auto weights = [&](auto mixed) {
+        const float ms = m == -INFINITY ? 0.f : m;
+        const float2 c2 = make_float2(p.qscale, p.qscale), m2 = make_float2(-ms, -ms);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint32_t s[64];
+        load_s(s);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, m2);
+          float2 w;
+          if constexpr (decltype(mixed)::value && Shape::kFmaOneIn > 0)
+            w = i % Shape::kFmaOneIn == 0 ? exp2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
+          else
+            w = make_float2(ex2(x.x), ex2(x.y));
+          sum[i & 1] = __fadd2_rn(sum[i & 1], w);
+          pk[i] = pack2<T>(w.x, w.y);
+        }
+        tile_sum = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      };
+      bool move = m == -INFINITY && n > 0;
+      if (!__any_sync(0xffffffffu, move)) {
+        if (ragged) weights(std::false_type{});
+        else weights(std::true_type{});
+        move = tile_sum > kMaxSum;
       }
-      float mx = -INFINITY;
+      if (__any_sync(0xffffffffu, move)) {
+        float mx = -INFINITY;
+        {
+          uint32_t s[64];
+          load_s(s);
 #pragma unroll
-      for (int i = 0; i < 64; ++i) mx = fmaxf(mx, __uint_as_float(s[i]));
-      mx *= p.qscale;
-      if (__any_sync(0xffffffffu, mx > m + kMaxSlack)) {
-        const float mn = fmaxf(m, mx), w = merge_weight(m, mn);
+          for (int i = 0; i < 64; i += 2) mx = max3(mx, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        }
+        const float mn = fmaxf(m, mx * p.qscale), w = merge_weight(m, mn);
         if (j > 0) {
           if (!wait_all(bars.pv, (uint32_t)((j - 1) & 1))) break;
           tc::fence_after_sync();
@@ -363,17 +434,10 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
           }
         }
         m = mn;
+        weights(std::false_type{});
       }
-      const float ms = m == -INFINITY ? 0.f : m;
-      uint32_t pk[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float a = ex2(fmaf(__uint_as_float(s[2 * i]), p.qscale, -ms));
-        const float c = ex2(fmaf(__uint_as_float(s[2 * i + 1]), p.qscale, -ms));
-        l += a + c;
-        pk[i] = pack2<T>(a, c);
-      }
-      tmem_st32(sp, pk);
+      l += tile_sum;
+      tmem_st32(sp, pk);  // over S, which has been read
       if (ragged) {
         // V rows that no query of the tile may see become zero; so do values that are
         // not finite in rows that only some of them see (added again at the end)
