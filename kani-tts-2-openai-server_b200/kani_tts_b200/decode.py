@@ -43,20 +43,44 @@ argmax, or, given ``SamplingParams``, the reference's penalty / top-k /
 temperature / top-p / multinomial sampler (inference_engine.py:349-430) as one
 ``sample_tokens`` launch per step, with the repetition history kept as a
 device bitmap and the Philox step counter advanced inside the graph.
+
+Streams of one voice may share their prompt's beginning (``set_prefix``): its keys
+and values are computed and kept once, the streams' prompts and steps attend to it
+through ``prefix_prefill_attention`` / ``prefix_decode_attention``.  With
+``DecodeEngine(cache_budget=...)`` generation outlives the static cache: the steps
+keep each row's accumulated attention weight, and a full cache is cut down to the
+budget (``evict_cache``).
 """
 from __future__ import annotations
+
+from dataclasses import dataclass, field
 
 import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .fused_kernels import (decode_advance, decode_attention, fused_add_rms_norm, fused_rms_norm,
+from .fused_kernels import (decode_advance, decode_attention, evict_cache, fused_add_rms_norm, fused_rms_norm,
                             fused_rope_kv_write, fused_silu_mul, gemm_tc, gemv, gemv_rope_kv_write, gemv_short_conv,
-                            head_argmax, head_argmax_tc, linear_split_k, reduce_add_rms_norm, sample_tokens,
-                            short_conv_step)
+                            head_argmax, head_argmax_tc, linear_split_k, prefix_decode_attention,
+                            prefix_prefill_attention, reduce_add_rms_norm, sample_tokens, short_conv_step)
 from .model import LFM2Config
-from .positions import learnable_inv_freq
+from .positions import frame_level_positions, learnable_inv_freq
 from .sampling import SamplingParams, seen_bitmap
+
+
+@dataclass
+class SharedPrefix:
+    """The beginning of the prompt that all streams share: keys and values per
+    attention layer [1, Hk, capacity, D], the conv states after it, its length on the
+    host and on the device, its tokens, and whether a speaker embedding is in it."""
+    k: dict
+    v: dict
+    conv: dict
+    length: int
+    device_length: torch.Tensor
+    tokens: torch.Tensor
+    speaker: bool = False
+    capacity: int = field(default=0)
 
 
 class FusedDecoder:
@@ -127,6 +151,8 @@ class FusedDecoder:
         self.conv_state = {i: torch.zeros(batch, h, cfg.conv_L_cache, dtype=self.dtype, device=dev)
                            for i, L in enumerate(self.layers) if not L["attn"]}
         self.err_flag = _lib.error_flag(dev)
+        self.prefix: SharedPrefix | None = None
+        self.scores: dict | None = None      # where steps add their attention weights (new_scores)
         # fused head + argmax: the CUDA-core GEMV kernel up to 8 streams (hidden 512 /
         # 1024 / 2048), the tensor-core kernel up to 64 (hidden a multiple of 64, at
         # most 1024); each keeps a cross-CTA argmax scratch that is zero between launches
@@ -242,6 +268,19 @@ class FusedDecoder:
     @property
     def dependent_attention(self) -> bool:
         return self.batch == 1 or not self.small_batch
+
+    def _attention(self, i: int, q_rot: torch.Tensor, kv_len: torch.Tensor) -> torch.Tensor:
+        """A decode step's attention of layer i, [B, Hq, D]: over the streams' own rows, or
+        behind the shared prefix and with accumulated weights where those are kept."""
+        if self.prefix is None and self.scores is None:
+            return decode_attention(q_rot, self.k_cache[i], self.v_cache[i], kv_len, self.scale,
+                                    err_flag=self.err_flag, prefix_final=self.dependent_attention)
+        p = self.prefix
+        return prefix_decode_attention(q_rot, self.k_cache[i], self.v_cache[i], kv_len,
+                                       None if p is None else p.k[i], None if p is None else p.v[i],
+                                       None if p is None else p.device_length, scale=self.scale,
+                                       scores=None if self.scores is None else self.scores[i],
+                                       err_flag=self.err_flag)
 
     # The norm prologue re-reads every stream's row in every CTA (from L2); beyond
     # this many streams a separate add + RMSNorm launch is cheaper (measured: equal
@@ -359,8 +398,7 @@ class FusedDecoder:
                                q_norm_w=L["q_norm"], k_norm_w=L["k_norm"], head_eps=self.eps,
                                frame_table=self.frame_table, tokens_per_frame=self.cfg.tokens_per_frame,
                                err_flag=self.err_flag, l2_prefetch=next(pf))
-                attn = decode_attention(q_rot, self.k_cache[i], self.v_cache[i], kv_len, self.scale,
-                                        err_flag=self.err_flag, prefix_final=self.dependent_attention)
+                attn = self._attention(i, q_rot, kv_len)
                 delta = gemv(attn.view(b, 1, self.q_dim), L["o"], l2_prefetch=next(pf))
             else:
                 y = normed(gemv_short_conv, L["in_proj"], self.conv_state[i], L["conv_w"], norm_weight=L["op_norm"],
@@ -419,8 +457,7 @@ class FusedDecoder:
                     self.k_cache[i], self.v_cache[i], slots, frame_table=self.frame_table,
                     tokens_per_frame=self.cfg.tokens_per_frame, q_norm_w=L["q_norm"], k_norm_w=L["k_norm"],
                     eps=self.eps, err_flag=self.err_flag)
-                attn = decode_attention(q_rot, self.k_cache[i], self.v_cache[i], kv_len, self.scale,
-                                        err_flag=self.err_flag, prefix_final=self.dependent_attention)   # [B, Hq, D]
+                attn = self._attention(i, q_rot, kv_len)   # [B, Hq, D]
                 delta = proj(attn.view(b, 1, self.q_dim), L["o"], self.split_k_out)
             else:
                 y = short_conv_step(F.linear(normed, L["in_proj"]), self.conv_state[i], L["conv_w"])
@@ -472,8 +509,7 @@ class FusedDecoder:
                     self.k_cache[i], self.v_cache[i], slots, frame_table=self.frame_table,
                     tokens_per_frame=self.cfg.tokens_per_frame, q_norm_w=L["q_norm"], k_norm_w=L["k_norm"],
                     eps=self.eps, err_flag=self.err_flag)
-                attn = decode_attention(q_rot, self.k_cache[i], self.v_cache[i], kv_len, self.scale,
-                                        err_flag=self.err_flag, prefix_final=self.dependent_attention)
+                attn = self._attention(i, q_rot, kv_len)
                 delta = proj(attn.view(b, 1, self.q_dim), L["o"])
             else:
                 bcx = gemm_tc(x_in, L["in_proj"], **norm_kw, **common)
@@ -510,8 +546,68 @@ class FusedDecoder:
         positions [B, T'] (T' = T + 1 with a speaker embedding, inserted at
         position 1 as inference_engine.py:475-491 does).  Fills KV slots
         0..T'-1 and the conv states; returns reduced-head logits of the last
-        token [B, 1, num_reduced]."""
-        b = self.batch
+        token [B, 1, num_reduced].  After ``set_prefix`` these are the tokens that
+        follow the shared prefix (positions counted from its beginning)."""
+        if speaker_emb is not None and self.prefix is not None:
+            raise ValueError("with a shared prefix the speaker embedding belongs to set_prefix")
+        return self._linear_head(self._prompt_pass(input_ids, positions, speaker_emb, self.batch, self.k_cache,
+                                                   self.v_cache, self.conv_state, self.prefix))
+
+    def set_prefix(self, input_ids: torch.Tensor, positions: torch.Tensor | None = None,
+                   speaker_emb: torch.Tensor | None = None, capacity: int | None = None) -> int:
+        """Compute the prompt's beginning once for all streams.
+
+        input_ids [P] or [1, P]; positions [1, P'] angle positions (default: as
+        ``DecodeEngine.start`` gives a prompt its positions); speaker_emb [1, dim] is
+        inserted at position 1.  Later ``prefill`` / ``step`` calls attend to it.
+        ``capacity`` (rows, default P') sizes its buffers: a later prefix that fits
+        them takes the same memory, so captured steps serve it without a new capture.
+        Returns P', the prefix's rows.
+        """
+        cfg, dev = self.cfg, self.device
+        ids = input_ids.reshape(1, -1).to(dev)
+        if ids.shape[1] == 0:
+            raise ValueError("an empty prefix: use clear_prefix")
+        rows = ids.shape[1] + (speaker_emb is not None)
+        if positions is None:
+            positions = _prompt_positions(cfg, ids, rows, speaker_emb is not None)
+        p = self.prefix
+        if p is None or rows > p.capacity or (capacity or 0) > p.capacity:
+            cap = max(rows, capacity or 0)
+            shape = (1, self.hk, cap, self.d)
+            k = {i: torch.zeros(shape, dtype=self.dtype, device=dev) for i in self.k_cache}
+            v = {i: torch.zeros(shape, dtype=self.dtype, device=dev) for i in self.v_cache}
+            conv = {i: torch.zeros_like(self.conv_state[i][:1]) for i in self.conv_state}
+            p = SharedPrefix(k, v, conv, 0, torch.zeros(1, dtype=torch.long, device=dev), ids, capacity=cap)
+        self._prompt_pass(ids, positions, speaker_emb, 1, p.k, p.v, p.conv, None, own_attention=True)
+        p.length, p.tokens, p.speaker = rows, ids, speaker_emb is not None
+        p.device_length.fill_(rows)
+        self.prefix = p
+        return rows
+
+    def clear_prefix(self) -> None:
+        """Back to prompts of their own (a step captured with a prefix needs a new capture)."""
+        self.prefix = None
+
+    def new_scores(self) -> dict:
+        """Zeroed accumulated weights [B, Hk, max_len] per attention layer.  Steps add to
+        them while they are assigned to ``scores``."""
+        return {i: torch.zeros(self.batch, self.hk, self.max_len, dtype=torch.float32, device=self.device)
+                for i in self.k_cache}
+
+    def evict(self, scores: dict, kv_len: torch.Tensor, budget: int, recent: int, protect: int) -> None:
+        """Cut every attention layer's caches down to `budget` rows, in place and by
+        `scores` (``evict_cache``); the new lengths are min(kv_len, budget)."""
+        for i in self.k_cache:
+            evict_cache(self.k_cache[i], self.v_cache[i], scores[i], kv_len, budget, recent, protect,
+                        err_flag=self.err_flag)
+
+    def _prompt_pass(self, input_ids, positions, speaker_emb, b, k_cache, v_cache, conv_state, prefix,
+                     own_attention: bool = False) -> torch.Tensor:
+        """A prompt of b streams through all layers into the given caches and conv
+        states, behind `prefix` where there is one: the last token's normed hidden state
+        [b, 1, H].  ``own_attention``: the library's causal attention also without a
+        prefix (SDPA otherwise)."""
         x = F.embedding(input_ids, self.embed)
         if speaker_emb is not None:
             spk = F.linear(speaker_emb.to(self.dtype), self.speaker_proj).unsqueeze(1)
@@ -520,6 +616,7 @@ class FusedDecoder:
         hq, hk, d = self.hq, self.hk, self.d
         slots = torch.arange(t, device=self.device, dtype=torch.long).repeat(b)
         pos = positions.reshape(-1).to(torch.long)
+        lens = torch.full((b,), t, dtype=torch.long, device=self.device) if prefix is not None or own_attention else None
         hidden, delta = x, None
         for i, L in enumerate(self.layers):
             if delta is None:
@@ -531,35 +628,75 @@ class FusedDecoder:
                 q, k, v = qkv.split([self.q_dim, self.kv_dim, self.kv_dim], dim=-1)
                 q_rot = fused_rope_kv_write(
                     q.view(b, t, hq, d), k.view(b, t, hk, d), v.view(b, t, hk, d), L["inv_freq"], pos,
-                    self.k_cache[i], self.v_cache[i], slots, frame_table=self.frame_table,
+                    k_cache[i], v_cache[i], slots, frame_table=self.frame_table,
                     tokens_per_frame=self.cfg.tokens_per_frame, q_norm_w=L["q_norm"], k_norm_w=L["k_norm"],
                     eps=self.eps, err_flag=self.err_flag)
-                rep = hq // hk                                    # prefill: expand K/V heads for GQA
-                attn = F.scaled_dot_product_attention(
-                    q_rot.transpose(1, 2), self.k_cache[i][:, :, :t].repeat_interleave(rep, dim=1),
-                    self.v_cache[i][:, :, :t].repeat_interleave(rep, dim=1),
-                    is_causal=True, scale=self.scale)                  # [B, Hq, T, D]
-                delta = F.linear(attn.transpose(1, 2).reshape(b, t, self.q_dim), L["o"])
+                if lens is not None:
+                    attn = prefix_prefill_attention(
+                        q_rot, k_cache[i], v_cache[i], lens, None if prefix is None else prefix.k[i],
+                        None if prefix is None else prefix.v[i], None if prefix is None else prefix.device_length,
+                        scale=self.scale, err_flag=self.err_flag)      # [B, T, Hq, D]
+                    delta = F.linear(attn.view(b, t, self.q_dim), L["o"])
+                else:
+                    rep = hq // hk                                    # prefill: expand K/V heads for GQA
+                    attn = F.scaled_dot_product_attention(
+                        q_rot.transpose(1, 2), k_cache[i][:, :, :t].repeat_interleave(rep, dim=1),
+                        v_cache[i][:, :, :t].repeat_interleave(rep, dim=1),
+                        is_causal=True, scale=self.scale)                  # [B, Hq, T, D]
+                    delta = F.linear(attn.transpose(1, 2).reshape(b, t, self.q_dim), L["o"])
             else:
                 bcx = F.linear(normed, L["in_proj"]).transpose(-1, -2)   # [B, 3H, T]
                 bg, c, xc = bcx.chunk(3, dim=-2)
                 bx = bg * xc
                 lc = self.cfg.conv_L_cache
-                self.conv_state[i].copy_(F.pad(bx, (lc - t, 0)) if t < lc else bx[..., t - lc:])
-                conv_out = F.conv1d(bx, L["conv_w"].unsqueeze(1), padding=lc - 1, groups=bx.shape[1])[..., :t]
+                if prefix is not None:
+                    # the conv goes on from the prefix's last inputs
+                    bx = torch.cat([prefix.conv[i].expand(b, -1, -1), bx], dim=-1)
+                    conv_out = F.conv1d(bx, L["conv_w"].unsqueeze(1), groups=bx.shape[1])[..., -t:]
+                    conv_state[i].copy_(bx[..., -lc:])
+                else:
+                    conv_state[i].copy_(F.pad(bx, (lc - t, 0)) if t < lc else bx[..., t - lc:])
+                    conv_out = F.conv1d(bx, L["conv_w"].unsqueeze(1), padding=lc - 1, groups=bx.shape[1])[..., :t]
                 delta = F.linear((c * conv_out).transpose(-1, -2), L["out_proj"])
             normed, hidden = fused_add_rms_norm(delta, hidden, L["ffn_norm"], self.eps)
             delta = F.linear(fused_silu_mul(F.linear(normed, L["gate_up"])), L["down"])
         normed, _ = fused_add_rms_norm(delta[:, -1:], hidden[:, -1:], self.final_norm, self.eps)
-        return self._linear_head(normed)
+        return normed
+
+
+def _prompt_positions(cfg, input_ids: torch.Tensor, rows: int, speaker: bool) -> torch.Tensor:
+    """[B, rows] angle positions of a prompt: frame-level ones, or sequential ones where a
+    speaker embedding is in it (inference_engine.py:497-499)."""
+    if speaker:
+        return torch.arange(rows, device=input_ids.device).repeat(input_ids.shape[0], 1)
+    return frame_level_positions(input_ids, cfg.audio_tokens_start, cfg.tokens_per_frame, cfg.audio_step).long()
 
 
 class DecodeEngine:
     """Prefill + CUDA-graph decode (greedy, or sampled with ``sampling``) for
-    `batch` independent streams."""
+    `batch` independent streams.
 
-    def __init__(self, decoder: FusedDecoder, keep_mask: bool = False, sampling: SamplingParams | None = None):
+    With ``cache_budget`` a full cache does not end generation: it is cut down to
+    that many rows per stream and KV head, which keep the prompt's own rows, the last
+    ``cache_recent`` rows (default: half of what the prompt leaves of the budget) and
+    the rows with the most accumulated attention weight.  The shared prefix of
+    ``FusedDecoder.set_prefix`` is never cut.
+    """
+
+    def __init__(self, decoder: FusedDecoder, keep_mask: bool = False, sampling: SamplingParams | None = None,
+                 cache_budget: int | None = None, cache_recent: int | None = None):
         self.dec = decoder
+        if cache_budget is not None and not 0 < cache_budget < decoder.max_len:
+            raise ValueError(f"cache_budget must lie between 0 and the cache's {decoder.max_len} rows")
+        if cache_budget is not None and keep_mask:
+            raise ValueError("an evicting engine keeps no additive mask")
+        if cache_recent is not None and (cache_budget is None or not 0 <= cache_recent <= cache_budget):
+            raise ValueError("cache_recent must lie between 0 and cache_budget")
+        self.cache_budget, self.cache_recent = cache_budget, cache_recent
+        self.scores = decoder.new_scores() if cache_budget is not None else None
+        self._filled = 0                 # own rows in the caches (every stream's)
+        self._prompt_rows = 0
+        self._captured_prefix = None
         self.keep_mask = keep_mask   # maintain the additive mask (for steps that use one)
         self.sampling = sampling
         dev, b, s = decoder.device, decoder.batch, decoder.max_len
@@ -583,33 +720,49 @@ class DecodeEngine:
         dec, cfg = self.dec, self.dec.cfg
         b, t = input_ids.shape
         t_eff = t + (1 if speaker_emb is not None else 0)
-        if t_eff + max_new_tokens > dec.max_len:
-            raise ValueError(f"cache of {dec.max_len} slots cannot hold {t_eff} + {max_new_tokens} tokens")
-        if speaker_emb is not None:   # speaker-conditioned prompts are sequential (inference_engine.py:497-499)
-            pos = torch.arange(t_eff, device=dec.device).repeat(b, 1)
+        if self.cache_budget is None:
+            if t_eff + max_new_tokens > dec.max_len:
+                raise ValueError(f"cache of {dec.max_len} slots cannot hold {t_eff} + {max_new_tokens} tokens")
+        elif t_eff + (self.cache_recent or 0) > self.cache_budget:
+            raise ValueError(f"a prompt of {t_eff} rows and {self.cache_recent or 0} recent ones do not fit a budget "
+                             f"of {self.cache_budget}")
+        history, before = input_ids, 0
+        if dec.prefix is None:
+            pos = _prompt_positions(cfg, input_ids, t_eff, speaker_emb is not None)
         else:
-            from .positions import frame_level_positions
-            pos = frame_level_positions(input_ids, cfg.audio_tokens_start, cfg.tokens_per_frame,
-                                        cfg.audio_step).long()
+            # the prompt is the prefix and these tokens: positions go on, the history is both
+            before = dec.prefix.length
+            history = torch.cat([dec.prefix.tokens.expand(b, -1), input_ids], dim=1)
+            pos = _prompt_positions(cfg, history, before + t_eff, dec.prefix.speaker)[:, before:]
+        for t in (self.scores or {}).values():
+            t.zero_()
         logits = dec.prefill(input_ids, pos, speaker_emb)
         self.rng_step.zero_()
         if self.sampling is not None:
             # the prompt is the initial repetition history (inference_engine.py:553-556)
-            self.seen = seen_bitmap(input_ids, dec.head.shape[0], dec.full_to_reduced, device=dec.device)
+            self.seen = seen_bitmap(history, dec.head.shape[0], dec.full_to_reduced, device=dec.device)
         first = self._next_token(logits[:, -1])
         self.rng_step.add_(1)
         self.input_ids.copy_(first.view(b, 1))
         self.mask.fill_(float("-inf"))
         self.mask[..., :t_eff] = 0.0
-        self.base_pos.fill_(t_eff)        # decode step k: t_eff + (k // tpf) * audio_step
+        self.base_pos.fill_(before + t_eff)   # decode step k: prompt length + (k // tpf) * audio_step
         self.base_slot.fill_(t_eff)       # decode step k writes slot t_eff + k
         self.step_idx.zero_()
         self.positions.copy_(self.base_pos)      # step 0; decode_advance computes the later ones
         self.slots.copy_(self.base_slot)
         self.kv_len.copy_(self.base_slot + 1)
         self.generated = torch.zeros(b, max_new_tokens, dtype=torch.long, device=dec.device)
+        self._filled = self._prompt_rows = t_eff
 
     def _step_body(self):
+        self.dec.scores = self.scores    # for this engine's steps alone
+        try:
+            self._step_launches()
+        finally:
+            self.dec.scores = None
+
+    def _step_launches(self):
         cfg = self.dec.cfg
         if self.keep_mask:
             self.mask.scatter_(3, self.slots.view(-1, 1, 1, 1), 0.0)
@@ -644,7 +797,8 @@ class DecodeEngine:
         saved = ({i: c.clone() for i, c in dec.conv_state.items()}, self.input_ids.clone(), self.mask.clone(),
                  self.step_idx.clone(), self.rng_step.clone(),
                  self.seen.clone() if self.seen is not None else None,
-                 self.positions.clone(), self.slots.clone(), self.kv_len.clone())
+                 self.positions.clone(), self.slots.clone(), self.kv_len.clone(),
+                 {i: t.clone() for i, t in (self.scores or {}).items()})
         s = torch.cuda.Stream(device=dec.device)
         s.wait_stream(torch.cuda.current_stream(dec.device))
         with torch.cuda.stream(s):
@@ -665,7 +819,25 @@ class DecodeEngine:
         self.positions.copy_(saved[6])
         self.slots.copy_(saved[7])
         self.kv_len.copy_(saved[8])
+        for i, t in saved[9].items():
+            self.scores[i].copy_(t)
+        self._captured_prefix = dec.prefix   # the graph reads its buffers
+
+    def _evict(self) -> None:
+        """Cut the full caches down to the budget; the next step writes behind what is left."""
+        budget, prompt = self.cache_budget, self._prompt_rows
+        recent = self.cache_recent if self.cache_recent is not None else (budget - prompt) // 2
+        self.dec.evict(self.scores, self.slots, budget, recent, prompt)      # slots: the rows written so far
+        cut = self._filled - budget
+        for t in (self.base_slot, self.slots, self.kv_len):
+            t.sub_(cut)
+        self._filled = budget
 
     def run(self, n_steps: int) -> None:
+        if self.dec.prefix is not self._captured_prefix:
+            raise RuntimeError("the shared prefix's buffers are not those of the captured step: capture() again")
         for _ in range(n_steps):
+            if self.cache_budget is not None and self._filled == self.dec.max_len:
+                self._evict()
             self.graph.replay()
+            self._filled += 1
