@@ -31,7 +31,8 @@ namespace cg = cooperative_groups;
 namespace kani {
 namespace {
 
-constexpr int kBins = 2048;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kBins = 2048, kDigits = kBins / kThreads;
 constexpr int kInFlight = 4;  // 16-byte pieces per thread and step
 
 struct EvictParams {
@@ -64,30 +65,28 @@ __device__ __forceinline__ uint32_t score_key(uint32_t u) {
 }
 
 // exclusive sum over the block's warps of one number per warp (given in all its
-// lanes), and the total; `red` holds WARPS ints
-template <int WARPS>
+// lanes), and the total; `red` holds kWarps ints
 __device__ __forceinline__ int warps_before(int x, int* red, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   __syncthreads();  // the last use of red is over
   if (lane == 0) red[warp] = x;
   __syncthreads();
-  int v = lane < WARPS ? red[lane] : 0, sum = v;
+  int v = lane < kWarps ? red[lane] : 0, sum = v;
 #pragma unroll
-  for (int o = 1; o < WARPS; o <<= 1) {
+  for (int o = 1; o < kWarps; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, sum, o);
     if (lane >= o) sum += y;
   }
-  total = __shfl_sync(0xffffffffu, sum, WARPS - 1);
+  total = __shfl_sync(0xffffffffu, sum, kWarps - 1);
   return __shfl_sync(0xffffffffu, sum - v, warp);
 }
 
-template <int THREADS, int ITEMS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) cache_evict_kernel(const EvictParams p) {
-  constexpr int WARPS = THREADS / 32, DIGITS = kBins / THREADS;
-  constexpr int CHUNK = THREADS * ITEMS;  // slots per chunk; warp w has ITEMS * 32 of them in a row
+template <int ITEMS>
+__global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const EvictParams p) {
+  constexpr int CHUNK = kThreads * ITEMS;  // slots per chunk; warp w has ITEMS * 32 of them in a row
   extern __shared__ int s_list[];               // kept slots of the chunk
   __shared__ int hist[kBins];
-  __shared__ int red[WARPS];
+  __shared__ int red[kWarps];
   __shared__ int s_digit, s_need;
   cg::cluster_group cluster = cg::this_cluster();
   const int ncl = (int)gridDim.x, rank = (int)blockIdx.x;
@@ -120,7 +119,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) cache_evict_kernel(co
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-      for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
+      for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
       __syncthreads();
 #pragma unroll 1
       for (int c = 0; c < chunks; ++c) {
@@ -134,11 +133,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) cache_evict_kernel(co
         }
       }
       __syncthreads();
-      // digits from the highest down: thread t has DIGITS of them
-      const int top = kBins - 1 - DIGITS * tid;
-      int mine[DIGITS], sum = 0;
+      // digits from the highest down: thread t has kDigits of them
+      const int top = kBins - 1 - kDigits * tid;
+      int mine[kDigits], sum = 0;
 #pragma unroll
-      for (int i = 0; i < DIGITS; ++i) sum += mine[i] = hist[top - i];
+      for (int i = 0; i < kDigits; ++i) sum += mine[i] = hist[top - i];
       int before = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -147,10 +146,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) cache_evict_kernel(co
       }
       int total;
       const int wsum = __shfl_sync(0xffffffffu, before, 31);
-      before += warps_before<WARPS>(wsum, red, total) - sum;
+      before += warps_before(wsum, red, total) - sum;
       if (before < need && need <= before + sum) {
 #pragma unroll
-        for (int i = 0; i < DIGITS; ++i) {
+        for (int i = 0; i < kDigits; ++i) {
           if (need > before && need <= before + mine[i]) {
             s_digit = top - i;
             s_need = need - before;
@@ -190,9 +189,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) cache_evict_kernel(co
       tied += __popc(__ballot_sync(0xffffffffu, mid && key == thr));
     }
     int all_tied, total;
-    int tie = tie0 + warps_before<WARPS>(tied, red, all_tied);  // tied rows before this warp's
+    int tie = tie0 + warps_before(tied, red, all_tied);  // tied rows before this warp's
     const int stay = sure + min(max(ties - tie, 0), tied);
-    int at = warps_before<WARPS>(stay, red, total);  // kept rows of the chunk before this warp's
+    int at = warps_before(stay, red, total);  // kept rows of the chunk before this warp's
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int j = slot(c, i);
@@ -225,12 +224,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) cache_evict_kernel(co
         w = w0 + (int)(i % wn);
       }
     };
-    for (int64_t i0 = 0; i0 < pieces; i0 += THREADS * kInFlight) {
+    for (int64_t i0 = 0; i0 < pieces; i0 += kThreads * kInFlight) {
       uint4 x[kInFlight];
       char* to[kInFlight];
 #pragma unroll
       for (int u = 0; u < kInFlight; ++u) {
-        const int64_t i = i0 + u * THREADS + tid;
+        const int64_t i = i0 + u * kThreads + tid;
         to[u] = nullptr;
         if (i < pieces) {
           int r, w;
@@ -255,24 +254,20 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) cache_evict_kernel(co
   }
   if (p.in_place && ncl > 1 && chunks == 0) cluster.sync();
   if (rank == 0) {
-    for (int64_t j = keep + tid; j < p.out_len; j += THREADS) so[j] = 0.f;
+    for (int64_t j = keep + tid; j < p.out_len; j += kThreads) so[j] = 0.f;
     if (kept)
-      for (int64_t j = keep + tid; j < p.budget; j += THREADS) kept[j] = -1;
+      for (int64_t j = keep + tid; j < p.budget; j += kThreads) kept[j] = -1;
     if (h == 0 && tid == 0) p.len_out[b] = keep;
   }
 }
 
-template <int THREADS, int ITEMS>
+template <int ITEMS>
 int launch_evict(const EvictParams& p, int ncl, int hk, int batch, cudaStream_t s) {
-  auto kern = cache_evict_kernel<THREADS, ITEMS>;
-  const size_t smem = (size_t)THREADS * ITEMS * sizeof(int);
-  if (smem > 32 * 1024) {
-    const cudaError_t a = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (a != cudaSuccess) return (int)a;
-  }
+  auto kern = cache_evict_kernel<ITEMS>;
+  const size_t smem = (size_t)kThreads * ITEMS * sizeof(int);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ncl, (unsigned)hk, (unsigned)batch);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -362,10 +357,10 @@ extern "C" int kani_cache_evict(int32_t dtype, int64_t batch, int32_t num_kv_hea
   int ncl = 1;
   while (ncl < 8 && batch * num_kv_heads * ncl * 2 <= 2 * sm_count() && ncl * 2 <= p.row_vecs) ncl *= 2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // one chunk where the cache allows it (measured: 64 x 8 caches of up to 2048 rows 59.7 us
-  // with 512 threads, 60.8 with 256, 69.0 with 1024; 16 x 4 of 8000 rows 64.8 us with 512,
-  // 67.8 with 1024; 8 x 2 of 16384 rows 75.5 us with 1024, 81.7 with 512)
-  if (cache_len <= 2048) return launch_evict<512, 4>(p, ncl, num_kv_heads, (int)batch, s);
-  if (cache_len <= 8192) return launch_evict<512, 16>(p, ncl, num_kv_heads, (int)batch, s);
-  return launch_evict<1024, 16>(p, ncl, num_kv_heads, (int)batch, s);
+  // Few slots per thread where the cache is short; chunks of 8192 where it is long.  (Blocks
+  // of 1024 threads, one chunk for 16384 slots, leave room for 15 clusters of 8 on the GPU:
+  // 8 x 2 caches of up to 16384 rows 75.2 us, with 512 threads 72.3; 64 x 8 caches of up to
+  // 2048 rows 59.7 us with 512 threads, 60.8 with 256, 69.0 with 1024.)
+  if (cache_len <= 2048) return launch_evict<4>(p, ncl, num_kv_heads, (int)batch, s);
+  return launch_evict<16>(p, ncl, num_kv_heads, (int)batch, s);
 }
