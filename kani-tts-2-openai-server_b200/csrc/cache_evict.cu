@@ -89,10 +89,13 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const EvictPar
   __shared__ int red[kWarps];
   __shared__ int s_digit, s_need;
   cg::cluster_group cluster = cg::this_cluster();
-  const int ncl = (int)gridDim.x, rank = (int)blockIdx.x;
+  const int ncl = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  // out of place, several clusters may share the kept rows of one (b, h); the first does the rest
+  const int parts = (int)gridDim.x / ncl, part = (int)blockIdx.x / ncl;
+  const bool lead = rank == 0 && part == 0;
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int64_t len = p.kv_len[b];
-  if ((len < 0 || len > p.cache_len) && rank == 0 && h == 0 && tid == 0 && p.err) atomicOr(p.err, KANI_FLAG_SLOT_OOB);
+  if ((len < 0 || len > p.cache_len) && lead && h == 0 && tid == 0 && p.err) atomicOr(p.err, KANI_FLAG_SLOT_OOB);
   const int n = (int)(len < 0 ? 0 : (len > p.cache_len ? p.cache_len : len));
   const bool cut = n > p.budget;
   const int keep = cut ? (int)p.budget : n;
@@ -203,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const EvictPar
       if (stays) {
         const int r = at + __popc(sm & below);
         s_list[r] = j;
-        if (rank == 0) {
+        if (lead) {
           so[dst0 + r] = __uint_as_float(raw[i]);
           if (kept) kept[dst0 + r] = j;
         }
@@ -214,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const EvictPar
     __syncthreads();  // the list is complete
 
     // pieces: index = row * wn + piece
-    const int64_t pieces = (int64_t)total * wn;
+    const int64_t first = (int64_t)total * part / parts * wn, pieces = (int64_t)total * (part + 1) / parts * wn;
     auto where = [&](int64_t i, int& r, int& w) {
       if (shift >= 0) {
         r = (int)(i >> shift);
@@ -224,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const EvictPar
         w = w0 + (int)(i % wn);
       }
     };
-    for (int64_t i0 = 0; i0 < pieces; i0 += kThreads * kInFlight) {
+    for (int64_t i0 = first; i0 < pieces; i0 += kThreads * kInFlight) {
       uint4 x[kInFlight];
       char* to[kInFlight];
 #pragma unroll
@@ -253,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const EvictPar
     if (c + 1 < chunks) __syncthreads();  // the list may be overwritten
   }
   if (p.in_place && ncl > 1 && chunks == 0) cluster.sync();
-  if (rank == 0) {
+  if (lead) {
     for (int64_t j = keep + tid; j < p.out_len; j += kThreads) so[j] = 0.f;
     if (kept)
       for (int64_t j = keep + tid; j < p.budget; j += kThreads) kept[j] = -1;
@@ -262,11 +265,11 @@ __global__ void __launch_bounds__(kThreads, 2) cache_evict_kernel(const EvictPar
 }
 
 template <int ITEMS>
-int launch_evict(const EvictParams& p, int ncl, int hk, int batch, cudaStream_t s) {
+int launch_evict(const EvictParams& p, int ncl, int parts, int hk, int batch, cudaStream_t s) {
   auto kern = cache_evict_kernel<ITEMS>;
   const size_t smem = (size_t)kThreads * ITEMS * sizeof(int);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ncl, (unsigned)hk, (unsigned)batch);
+  cfg.gridDim = dim3((unsigned)(ncl * parts), (unsigned)hk, (unsigned)batch);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -356,11 +359,20 @@ extern "C" int kani_cache_evict(int32_t dtype, int64_t batch, int32_t num_kv_hea
   // enough CTAs for two per SM, each with 32 bytes or more of a row
   int ncl = 1;
   while (ncl < 8 && batch * num_kv_heads * ncl * 2 <= 2 * sm_count() && ncl * 2 <= p.row_vecs) ncl *= 2;
+  // in place a cluster's columns are all the split there is; elsewhere more clusters may
+  // share the rows, each after a selection of its own, while 128 KB are left to each CTA
+  // (8 x 2 caches, 4 MB kept of each: 72.2 us alone, 62.4 with two; one stream's 8 x 128 KB:
+  // 7.2 us alone, 9.8 with four)
+  int parts = 1;
+  if (!in_place && ncl == 8)
+    while (parts < 4 && batch * num_kv_heads * ncl * parts * 2 <= 2 * sm_count() &&
+           budget * p.row_vecs * 32 / (ncl * parts * 2) >= 128 << 10)
+      parts *= 2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // Few slots per thread where the cache is short; chunks of 8192 where it is long.  (Blocks
   // of 1024 threads, one chunk for 16384 slots, leave room for 15 clusters of 8 on the GPU:
   // 8 x 2 caches of up to 16384 rows 75.2 us, with 512 threads 72.3; 64 x 8 caches of up to
   // 2048 rows 59.7 us with 512 threads, 60.8 with 256, 69.0 with 1024.)
-  if (cache_len <= 2048) return launch_evict<4>(p, ncl, num_kv_heads, (int)batch, s);
-  return launch_evict<16>(p, ncl, num_kv_heads, (int)batch, s);
+  if (cache_len <= 2048) return launch_evict<4>(p, ncl, parts, num_kv_heads, (int)batch, s);
+  return launch_evict<16>(p, ncl, parts, num_kv_heads, (int)batch, s);
 }
