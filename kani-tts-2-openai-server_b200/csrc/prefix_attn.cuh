@@ -65,6 +65,10 @@ inline int check_params(Params& p, int32_t dtype, int64_t batch, int64_t tokens,
   if (hk == 1) p.ch = p.ph = p.sh = 0;
   if (p.cache_len <= 1) p.cs = 0;
   if (p.prefix_rows <= 1) p.ps = 0;
+  // rows, heads and queries that are one and the same memory make no tensor map
+  if ((p.cs == 0 && p.cache_len > 1) || (p.ps == 0 && p.prefix_rows > 1) || (p.qh == 0 && hq > 1) ||
+      (p.qt == 0 && tokens > 1))
+    return KANI_ERR_UNSUPPORTED;
   for (int64_t x : {p.qb, p.qt, p.qh, p.cb, p.ch, p.cs, p.ph, p.ps, p.ob, p.ot, p.oh})
     if (x % 8 != 0) return KANI_ERR_UNSUPPORTED;
   for (const void* x : {p.q, p.k, p.v, p.pk, p.pv, (const void*)p.out})

@@ -15,7 +15,7 @@
 //     tensor-memory buffers, so the next S is computed while this one is worked on)
 //     and O += P V with P taken from tensor memory and V as it lies (rows = keys: an
 //     MN-major operand);
-//   * warps 0..3 hold one query row per thread: maximum, p = 2^(s c - m), sum in
+//   * warps 0..3 hold one query row per thread: p = 2^(s c - m) and their sum in
 //     fp32; P is rounded to the storage type (bf16 / fp16: half a step of it relative
 //     to each weight, as the result's own rounding) and replaces S in tensor memory.
 // The running maximum moves only when a tile's weights sum to more than 2^10, so most
@@ -175,13 +175,21 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// 2^x on the FMA pipes, for x < 128: x = n + f with n the nearest integer (read off the
-// low bits of x + 1.5 * 2^23), 2^f by a polynomial of degree 4 fitted to the least
-// relative error on [-1/2, 1/2] (2.7e-6, under a hundredth of half a step of fp16), n
-// added to the exponent.  Below 2^-126 it stays there.
+// 2^x on the FMA pipes: x = n + f with n the nearest integer (read off the low bits of
+// x + 1.5 * 2^23), 2^f by a polynomial of degree 4 fitted to the least relative error on
+// [-1/2, 1/2] (2.7e-6, under a hundredth of half a step of fp16), n added to the
+// exponent.  x is held to [-126, 127]: what lies below counts as 2^-126, what lies above
+// is far past kMaxSum and is done again.  A NaN stays one up to the last step, where its
+// bits (0x7fffffff, as the arithmetic makes them) give the largest finite number: past
+// kMaxSum too.
+__device__ __forceinline__ float clamp_exponent(float x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-126.f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(127.f));
+  return x;
+}
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
+  x.x = clamp_exponent(x.x);
+  x.y = clamp_exponent(x.y);
   const float2 magic = make_float2(12582912.f, 12582912.f);
   const float2 t = __fadd2_rn(x, magic);
   const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
@@ -245,8 +253,6 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   griddep_wait();
-  // only now: a dependent of this launch may rely on the launches before it
-  griddep_launch_dependents();
 
   const bool tell = tid == 0 && blockIdx.x == 0 && h == 0;
   const int plen = p.prefix_len ? checked_len(*p.prefix_len, p.prefix_rows, p.err, tell && b == 0) : p.prefix_rows;
@@ -269,6 +275,9 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = s_tmem;
+  // only now: a dependent of this launch may rely on the launches before it, and one that
+  // needs tensor memory must not come between this block and its own
+  griddep_launch_dependents();
 
   // n finished (or, for partials, unnormalised) columns from c on of the tile's row r
   auto store = [&](int r, int c, float2 ml, const float* f, int n) {
@@ -617,8 +626,7 @@ int launch_flash(const Params& p, int32_t dtype, int d, int batch, int tokens, b
   memset(&f, 0, sizeof(f));
   f.tpt = kRows / p.group;
   // the expanded dimensions (stride 0) of Q and the caches are one element to the copies
-  const bool qb = batch > 1 && p.qb != 0, qt_one = p.qt == 0 && tokens > 1, qh_one = p.qh == 0 && p.hq > 1;
-  if (qt_one || qh_one || (p.cs == 0 && p.cache_len > 1) || (p.ps == 0 && p.prefix_rows > 1)) return KANI_ERR_UNSUPPORTED;
+  const bool qb = batch > 1 && p.qb != 0;
   f.qb_step = qb;
   f.b_step = p.cb != 0;
   f.h_step = p.ch != 0;

@@ -1162,7 +1162,8 @@ def _attention_scale(scale, d: int) -> float:
 
 @functools.lru_cache(maxsize=1024)
 def _prefix_workspace_bytes(device_index: int, *sizes: int) -> int:
-    return int(load_library().kani_prefix_decode_workspace(*sizes))
+    with torch.cuda.device(device_index):      # the split depends on the device's SMs
+        return int(load_library().kani_prefix_decode_workspace(*sizes))
 
 
 def _prefix_workspace(device: torch.device, index: int, *sizes: int):
@@ -1215,6 +1216,8 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     qv = q.squeeze(1) if q.dim() == 4 and q.shape[1] == 1 else q
     if qv.dim() != 3 or qv.shape[0] != b or qv.shape[2] != d or (qv.stride(2) != 1 and qv.numel()):
         raise ValueError(f"q must be [{b}, heads, {d}] with a contiguous last dim")
+    if 0 in qv.stride():
+        qv = qv.contiguous()        # (expanded over streams or heads)
     qb, qh, _ = qv.stride()
     hq = qv.shape[1]
     if hk == 0 or hq % hk:
@@ -1289,6 +1292,8 @@ def prefix_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
             raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)}")
         _refuse_overlap(((out, "out"),), ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (pk, "prefix_k"),
                                           (pv, "prefix_v"), (kv_len, "kv_len"), (q_len, "q_len")))
+    if 0 in q.stride():
+        q = q.contiguous()          # (expanded over streams, tokens or heads)
     qs = q.stride()
     _call(index, "kani_prefix_prefill_attention", lib.kani_prefix_prefill_attention,
           code, b, t, hq, hk, d, q.data_ptr(), qs[0], qs[1], qs[2], k_cache.data_ptr(), v_cache.data_ptr(), cs[0],

@@ -3,8 +3,9 @@
 Bounds.  Inputs are exact.  A logit is an fp32 sum of D exact products, scaled once:
 it is off by at most (D + 2) 2^-24 sum|q k| scale; its exponential's argument, at most
 2 dot log2(e) in magnitude, is rounded to 2^-24 of it, twice, and the hardware's 2^x is
-off by 2^-22.  So every weight, and their sum, is off by a factor within 1 +- r with
-    r = (D + 2) 2^-24 dot + 8 dot 2^-24 + 2^-21 + N 2^-24
+off by 2^-22 (the polynomial that replaces it for some weights by 2.7e-6 < 2^-18).  So
+every weight, and their sum, is off by a factor within 1 +- r with
+    r = (D + 2) 2^-24 dot + 8 dot 2^-24 + 2^-18 + N 2^-24
 (the last term: sums over N rows), and the output by 2 r mass, mass = sum w |v|.  Weights
 may be rounded to the storage type before they meet V: u mass more, u = eps / 2 of that
 type.  The result is rounded once: u |out|.  fp16 adds half its smallest subnormal, 2^-25,
@@ -27,7 +28,7 @@ DEV = "cuda"
 
 
 def rel_bound(dot, d, n):
-    return (d + 2) * 2.0 ** -24 * dot + 8 * dot * 2.0 ** -24 + 2.0 ** -21 + n * 2.0 ** -24
+    return (d + 2) * 2.0 ** -24 * dot + 8 * dot * 2.0 ** -24 + 2.0 ** -18 + n * 2.0 ** -24
 
 
 def check_out(got, ref, mass, dot, n, vmax):
@@ -255,6 +256,64 @@ def test_prefill_does_not_see_later_rows(bad):
         assert (later[..., 5] == bad).all()
         assert (later[:, 80 - first:, :, 9] == bad).all()
         assert torch.isfinite(later[:, :80 - first, :, 9]).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("what", ["nan", "inf", "spike", "huge spike"])
+def test_one_odd_key_at_every_place(what, d):
+    """A single key of the prefix at each place of a tile, seen by every query: a NaN or
+    infinite one makes every result NaN (an infinite logit has no softmax), one whose logit
+    exceeds the others by 60 or by hundreds of powers of two owns the result."""
+    g = torch.Generator().manual_seed(77)
+    dt = torch.bfloat16
+    p, n = 192, 64
+    q = torch.ones(n, 5, 2, d, dtype=dt)                       # a stream per place, 5 tokens each
+    k, v = make((n, 1, 5, d), g, dt), make((n, 1, 5, d), g, dt)
+    pk, pv = make((1, p, d), g, dt), make((1, p, d), g, dt)
+    dev = [x.to(DEV) for x in (q, k, v, torch.full((n,), 5), pk, pv)]
+    size = {"nan": float("nan"), "inf": float("inf"), "spike": 60 * math.log(2) / d, "huge spike": 400.0 / d}[what]
+    for place in range(64, 128):
+        bad = dev[4].clone()
+        bad[0, place] = size
+        out = K.prefix_prefill_attention(dev[0][:1], dev[1][:1], dev[2][:1], dev[3][:1], bad, dev[5], scale=1.0)
+        dec = K.prefix_decode_attention(dev[0][:, 0], dev[1], dev[2], dev[3], bad.expand(1, p, d), dev[5], scale=1.0)
+        if what in ("nan", "inf"):
+            assert out.isnan().all() and dec.isnan().all()
+        else:
+            ref, mass, dot = O.prefix_prefill_attention(q[:1, :1], k[:1], v[:1], [1], [1], bad.cpu(), pv, p, 1.0)
+            check_out(out[:, :1], ref, mass, dot, p + 5, 6.0)
+            ref, mass, dot, _ = O.prefix_decode_attention(q[:1, 0], k[:1], v[:1], [5], bad.cpu(), pv, p, 1.0)
+            check_out(dec[:1], ref, mass, dot, p + 5, 6.0)
+
+
+def test_logits_that_keep_growing():
+    """Each tile's logits exceed the last one's, by a little and by hundreds: the running
+    maximum moves tile after tile."""
+    g = torch.Generator().manual_seed(78)
+    for step in (0.4, 5.0, 60.0):
+        p, d, b = 700, 64, 70
+        q = torch.ones(1, b, 2, d, dtype=torch.bfloat16)
+        pk = (torch.arange(p).view(1, p, 1) * step / 64 / d + 0.01 * torch.randn(1, p, d, generator=g)).bfloat16()
+        pv, k, v = make((1, p, d), g, torch.bfloat16), make((1, 1, b, d), g, torch.bfloat16), make((1, 1, b, d), g, torch.bfloat16)
+        ref, mass, dot = O.prefix_prefill_attention(q, k, v, [b], [b], pk, pv, p, 1.0)
+        out = K.prefix_prefill_attention(*(x.to(DEV) for x in (q, k, v, torch.tensor([b]), pk, pv)), scale=1.0)
+        check_out(out, ref, mass, dot, p + b, 6.0)
+
+
+def test_expanded_inputs():
+    """Queries and caches expanded over streams or heads give what their copies give."""
+    g = torch.Generator().manual_seed(79)
+    dt = torch.bfloat16
+    q = make((1, 3, 4, 64), g, dt).to(DEV).expand(5, 3, 4, 64)
+    k, v = (make((1, 1, 40, 64), g, dt).to(DEV).expand(5, 2, 40, 64) for _ in range(2))
+    pk, pv = (make((1, 200, 64), g, dt).to(DEV).expand(2, 200, 64) for _ in range(2))
+    n = torch.tensor([40, 3, 17, 30, 8], device=DEV)
+    a = K.prefix_prefill_attention(q, k, v, n, pk, pv)
+    assert torch.equal(a, K.prefix_prefill_attention(*(x.contiguous() for x in (q, k, v, n, pk, pv))))
+    a = K.prefix_decode_attention(q[:, 0], k, v, n, pk, pv)
+    assert torch.equal(a, K.prefix_decode_attention(*(x.contiguous() for x in (q[:, 0], k, v, n, pk, pv))))
+    with pytest.raises(_lib.KaniError):
+        K.prefix_decode_attention(q[:, 0], k[:, :, :1].expand(5, 2, 40, 64), v[:, :, :1].expand(5, 2, 40, 64), n)
 
 
 def test_prefill_strided_and_chunked():
