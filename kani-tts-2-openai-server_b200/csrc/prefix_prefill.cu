@@ -56,10 +56,10 @@ constexpr int kMaxStages = 4;
 template <int D> struct FlashShape {
   static constexpr int kStages = D == 64 ? 4 : 2;
   // One pair of weights in so many by polynomial instead of the special-function unit,
-  // which takes 8 cycles for a warp's 32: with D = 64 that unit bounds the kernel (4 x
-  // 4096 tokens behind 4096 rows: none 610 us, one in 4 552, one in 3 555), with D = 128
-  // the products weigh twice as much (3 x 777 tokens: none 55.7 us, one in 4 58.0).
-  static constexpr int kFmaOneIn = D == 64 ? 4 : 0;
+  // which takes 8 cycles for a warp's 32: with D = 64 that unit is the busiest (4 x 4096
+  // tokens behind 4096 rows: none 610 us, one in 4 565, one in 6 552, one in 8 557), with
+  // D = 128 the products weigh twice as much (3 x 777 tokens: none 55.7 us, one in 4 58.0).
+  static constexpr int kFmaOneIn = D == 64 ? 6 : 0;
   static constexpr uint32_t kQBytes = kRows * D * 2;
   static constexpr uint32_t kTileBytes = kKeys * D * 2;
   // 2 CTAs per SM by shared memory, so two blocks' 256 columns fill tensor memory
