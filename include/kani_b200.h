@@ -547,6 +547,22 @@ KANI_API int kani_prefix_decode_attention(int32_t dtype, int64_t batch, int32_t 
                      int64_t scores_head_stride, void* out, int64_t out_batch_stride,
                      int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
                      int32_t* err_flag, void* stream);
+/*
+ * The same call of one decode step, launched as a programmatic dependent: kv_len, the
+ * prefix and the rows below kv_len - 1 must be final before the launch ahead of it on the
+ * stream, which may write q and each stream's newest row, kv_len - 1.  Those are read after
+ * that launch has completed, the older rows stream in while it runs.  Same results.
+ */
+KANI_API int kani_prefix_decode_attention_step(int32_t dtype, int64_t batch, int32_t num_q_heads,
+                     int32_t num_kv_heads, int32_t head_dim, const void* q, int64_t q_batch_stride,
+                     int64_t q_head_stride, const void* k_cache, const void* v_cache,
+                     int64_t cache_batch_stride, int64_t cache_head_stride, int64_t cache_slot_stride,
+                     int64_t cache_len, const int64_t* kv_len, const void* prefix_k, const void* prefix_v,
+                     int64_t prefix_head_stride, int64_t prefix_row_stride, int64_t prefix_rows,
+                     const int64_t* prefix_len, float scale, float* scores, int64_t scores_batch_stride,
+                     int64_t scores_head_stride, void* out, int64_t out_batch_stride,
+                     int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
+                     int32_t* err_flag, void* stream);
 
 /*
  * The prompt pass of the same attention: query i < q_len[b] of stream b (q_len NULL:

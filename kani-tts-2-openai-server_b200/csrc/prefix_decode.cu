@@ -51,6 +51,7 @@ struct DecodeParams : Params {
   float* logits;     // workspace [B, Hq, cache_len] when they do not fit in shared memory
   int logit_rows;    // else rows per CTA
   int by_length;     // blocks take the streams in the order of their lengths
+  int step;          // launched as a programmatic dependent of the launch that writes q and the newest rows
   int parts;         // the prefix's partials (0: this kernel reads the prefix rows itself)
   const float* acc;  // [parts][B, Hq][D]
   const float* ml;   // [parts][B, Hq][2]
@@ -196,11 +197,21 @@ __global__ void __launch_bounds__(kThreads) prefix_decode_kernel(const __grid_co
     }
   };
   const int nit = (wn + KEYS - 1) / KEYS;
+  auto first_steps = [&] {
 #pragma unroll
-  for (int it = 0; it < STAGES - 1; ++it) {
-    if (it < nit) issue(it);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
+    for (int it = 0; it < STAGES - 1; ++it) {
+      if (it < nit) issue(it);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  // As a step's dependent launch (p.step), the first rows stream in while the launch
+  // before still runs, but in the warp where they hold the stream's newest row, the one
+  // which that launch may be writing.
+  const bool newest = no > 0 && o0 + no == own && w0 + wn == n;
+  const bool early = p.step && !(newest && nit < STAGES);
+  if (early) first_steps();
+  if (p.step) griddep_wait();  // q and the newest row
+  if (!early) first_steps();
 
   // Q as the A operand: head g's dims 2 t4.. of each 16-wide step (rows 8..15 are zero)
   uint32_t qa[D / 16][2];
@@ -405,7 +416,7 @@ int launch_decode(DecodeParams& p, int ncl, cudaStream_t s) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.parts ? 2 : 1;
+  cfg.numAttrs = p.parts || p.step ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   note_launch();
   return e == cudaSuccess ? KANI_OK : (int)e;
@@ -455,14 +466,16 @@ extern "C" int64_t kani_prefix_decode_workspace(int64_t batch, int32_t num_q_hea
   return p.logits + p.acc + p.ml;
 }
 
-extern "C" int kani_prefix_decode_attention(
+namespace {
+int prefix_decode_impl(
     int32_t dtype, int64_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, const void* q,
     int64_t q_batch_stride, int64_t q_head_stride, const void* k_cache, const void* v_cache,
     int64_t cache_batch_stride, int64_t cache_head_stride, int64_t cache_slot_stride, int64_t cache_len,
     const int64_t* kv_len, const void* prefix_k, const void* prefix_v, int64_t prefix_head_stride,
     int64_t prefix_row_stride, int64_t prefix_rows, const int64_t* prefix_len, float scale, float* scores,
     int64_t scores_batch_stride, int64_t scores_head_stride, void* out, int64_t out_batch_stride,
-    int64_t out_head_stride, void* workspace, int64_t workspace_bytes, int32_t* err_flag, void* stream) {
+    int64_t out_head_stride, void* workspace, int64_t workspace_bytes, int32_t* err_flag, void* stream,
+    bool step) {
   using namespace kani;
   if (batch < 0 || num_q_heads < 0 || num_kv_heads < 0 || head_dim < 0 || cache_len < 0 || prefix_rows < 0 ||
       workspace_bytes < 0)
@@ -503,6 +516,8 @@ extern "C" int kani_prefix_decode_attention(
   p.acc = acc;
   p.ml = ml;
   p.parts = plan.parts;
+  // behind the prefix launch, which itself waits for the launch before, nothing is pending
+  p.step = step && !plan.parts;
   // Finding a block's place costs it up to 0.4 us: worth it while the blocks make few
   // waves (64 streams x 8 heads), not for more (128 x 8, 20 rows each: 24.1 us without
   // it, 26.8 with).
@@ -514,12 +529,49 @@ extern "C" int kani_prefix_decode_attention(
     prefix::Params f = p;
     f.qt = p.qb;
     f.qb = 0;
-    const int rc = prefix::launch_flash(f, dtype, head_dim, 1, (int)batch, false, plan.split, ml, acc, s);
+    const int rc = prefix::launch_flash(f, dtype, head_dim, 1, (int)batch, false, plan.split, ml, acc, step, s);
     if (rc != KANI_OK) return rc;
   }
   auto go = [&]<typename T>() {
-    // rings of 64 KB (three blocks per SM); deeper or finer ones measured up to 20 % slower
-    return head_dim == 64 ? launch_decode<T, 64, 32, 2>(p, plan.ncl, s) : launch_decode<T, 128, 16, 2>(p, plan.ncl, s);
+    // Rings of 64 KB, three blocks per SM; of 48 KB where those make two waves of the blocks
+    // and four per SM make one (64 streams of 880 rows: 30.3 us with 64 KB, 23.8 with 48;
+    // behind a prefix launch, which takes the shared memory of one, 25.7 and 28.6).
+    const int64_t blocks = batch * num_kv_heads * plan.ncl;
+    const bool small = !plan.parts && blocks > 3 * sm_count() && blocks <= 4 * sm_count();
+    if (head_dim == 64)
+      return small ? launch_decode<T, 64, 16, 3>(p, plan.ncl, s) : launch_decode<T, 64, 32, 2>(p, plan.ncl, s);
+    return launch_decode<T, 128, 16, 2>(p, plan.ncl, s);
   };
   return dtype == KANI_DTYPE_BF16 ? go.template operator()<__nv_bfloat16>() : go.template operator()<__half>();
+}
+}  // namespace
+
+extern "C" int kani_prefix_decode_attention(
+    int32_t dtype, int64_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, const void* q,
+    int64_t q_batch_stride, int64_t q_head_stride, const void* k_cache, const void* v_cache,
+    int64_t cache_batch_stride, int64_t cache_head_stride, int64_t cache_slot_stride, int64_t cache_len,
+    const int64_t* kv_len, const void* prefix_k, const void* prefix_v, int64_t prefix_head_stride,
+    int64_t prefix_row_stride, int64_t prefix_rows, const int64_t* prefix_len, float scale, float* scores,
+    int64_t scores_batch_stride, int64_t scores_head_stride, void* out, int64_t out_batch_stride,
+    int64_t out_head_stride, void* workspace, int64_t workspace_bytes, int32_t* err_flag, void* stream) {
+  return prefix_decode_impl(dtype, batch, num_q_heads, num_kv_heads, head_dim, q, q_batch_stride, q_head_stride, k_cache, v_cache,
+                            cache_batch_stride, cache_head_stride, cache_slot_stride, cache_len, kv_len, prefix_k,
+                            prefix_v, prefix_head_stride, prefix_row_stride, prefix_rows, prefix_len, scale, scores,
+                            scores_batch_stride, scores_head_stride, out, out_batch_stride, out_head_stride, workspace,
+                            workspace_bytes, err_flag, stream, false);
+}
+
+extern "C" int kani_prefix_decode_attention_step(
+    int32_t dtype, int64_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, const void* q,
+    int64_t q_batch_stride, int64_t q_head_stride, const void* k_cache, const void* v_cache,
+    int64_t cache_batch_stride, int64_t cache_head_stride, int64_t cache_slot_stride, int64_t cache_len,
+    const int64_t* kv_len, const void* prefix_k, const void* prefix_v, int64_t prefix_head_stride,
+    int64_t prefix_row_stride, int64_t prefix_rows, const int64_t* prefix_len, float scale, float* scores,
+    int64_t scores_batch_stride, int64_t scores_head_stride, void* out, int64_t out_batch_stride,
+    int64_t out_head_stride, void* workspace, int64_t workspace_bytes, int32_t* err_flag, void* stream) {
+  return prefix_decode_impl(dtype, batch, num_q_heads, num_kv_heads, head_dim, q, q_batch_stride, q_head_stride, k_cache, v_cache,
+                            cache_batch_stride, cache_head_stride, cache_slot_stride, cache_len, kv_len, prefix_k,
+                            prefix_v, prefix_head_stride, prefix_row_stride, prefix_rows, prefix_len, scale, scores,
+                            scores_batch_stride, scores_head_stride, out, out_batch_stride, out_head_stride, workspace,
+                            workspace_bytes, err_flag, stream, true);
 }

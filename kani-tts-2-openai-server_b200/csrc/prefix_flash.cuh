@@ -18,9 +18,9 @@ FlashSplit flash_split(int64_t batch, int64_t tokens, int hq, int hk, int64_t ro
 // alone, of all of batch x tokens queries.  ml / acc: partials [parts][rows][2] and
 // [parts][rows][D] (fp32; maximum in powers of 2, sum, unnormalised output; a sum of
 // 0 = no row seen, with an output of zeros); NULL (one part only): the result goes to
-// p.out.
+// p.out.  dependent: as a programmatic dependent of the launch before it.
 int launch_flash(const Params& p, int32_t dtype, int d, int batch, int tokens, bool own_rows, FlashSplit split,
-                 float* ml, float* acc, cudaStream_t s);
+                 float* ml, float* acc, bool dependent, cudaStream_t s);
 
 }  // namespace prefix
 }  // namespace kani

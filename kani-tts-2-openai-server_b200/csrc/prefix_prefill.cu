@@ -598,7 +598,7 @@ FlashSplit flash_split(int64_t batch, int64_t tokens, int hq, int hk, int64_t ro
 }
 
 template <typename T, int D>
-static int launch_flash_t(const FlashParams& f, int hk, int batch, cudaStream_t s) {
+static int launch_flash_t(const FlashParams& f, int hk, int batch, bool dependent, cudaStream_t s) {
   auto kern = prefix_flash_kernel<T, D>;
   static std::atomic<uint64_t> granted{0};
   if (const int e = grant_smem(kern, FlashShape<D>::kSmem, granted)) return e;
@@ -607,20 +607,22 @@ static int launch_flash_t(const FlashParams& f, int hk, int batch, cudaStream_t 
   cfg.blockDim = dim3(kFlashThreads);
   cfg.dynamicSmemBytes = FlashShape<D>::kSmem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)f.cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = dependent ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, f);
   note_launch();
   return e == cudaSuccess ? KANI_OK : (int)e;
 }
 
 int launch_flash(const Params& p, int32_t dtype, int d, int batch, int tokens, bool own_rows, FlashSplit split,
-                 float* ml, float* acc, cudaStream_t s) {
+                 float* ml, float* acc, bool dependent, cudaStream_t s) {
   const bool bf16 = dtype == KANI_DTYPE_BF16;
   FlashParams f;
   memset(&f, 0, sizeof(f));
@@ -667,10 +669,10 @@ int launch_flash(const Params& p, int32_t dtype, int d, int batch, int tokens, b
   f.prefix_rows = (int)p.prefix_rows;
   f.cache_len = own_rows ? (int)p.cache_len : 0;
   if (bf16)
-    return d == 64 ? launch_flash_t<__nv_bfloat16, 64>(f, p.hk, batch, s)
-                   : launch_flash_t<__nv_bfloat16, 128>(f, p.hk, batch, s);
-  return d == 64 ? launch_flash_t<__half, 64>(f, p.hk, batch, s)
-                 : launch_flash_t<__half, 128>(f, p.hk, batch, s);
+    return d == 64 ? launch_flash_t<__nv_bfloat16, 64>(f, p.hk, batch, dependent, s)
+                   : launch_flash_t<__nv_bfloat16, 128>(f, p.hk, batch, dependent, s);
+  return d == 64 ? launch_flash_t<__half, 64>(f, p.hk, batch, dependent, s)
+                 : launch_flash_t<__half, 128>(f, p.hk, batch, dependent, s);
 }
 
 }  // namespace prefix
@@ -717,5 +719,5 @@ extern "C" int kani_prefix_prefill_attention(
     return bad;
   return prefix::launch_flash(p, dtype, head_dim, (int)batch, (int)tokens, true,
                               prefix::flash_split(batch, tokens, num_q_heads, num_kv_heads, prefix_rows + cache_len, 1),
-                              nullptr, nullptr, static_cast<cudaStream_t>(stream));
+                              nullptr, nullptr, false, static_cast<cudaStream_t>(stream));
 }

@@ -101,6 +101,7 @@ _SIGNATURES = {
                                       _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_f32,
                                       _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p],
                                      ctypes.c_int),
+    "kani_prefix_decode_attention_step": None,     # as above, set below
     "kani_prefix_prefill_attention": ([_c_i32, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_i64, _c_i64, _c_i64,
                                        _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p,
                                        _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_f32,
@@ -110,6 +111,8 @@ _SIGNATURES = {
                           _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p,
                           _c_p, _c_p, _c_p], ctypes.c_int),
 }
+
+_SIGNATURES["kani_prefix_decode_attention_step"] = _SIGNATURES["kani_prefix_decode_attention"]
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 

@@ -280,7 +280,7 @@ class FusedDecoder:
                                        None if p is None else p.k[i], None if p is None else p.v[i],
                                        None if p is None else p.device_length, scale=self.scale,
                                        scores=None if self.scores is None else self.scores[i],
-                                       err_flag=self.err_flag)
+                                       err_flag=self.err_flag, prefix_final=self.dependent_attention)
 
     # The norm prologue re-reads every stream's row in every CTA (from L2); beyond
     # this many streams a separate add + RMSNorm launch is cheaper (measured: equal

@@ -1186,7 +1186,7 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                             prefix_k: torch.Tensor | None = None, prefix_v: torch.Tensor | None = None,
                             prefix_len: torch.Tensor | None = None, *, scale: float | None = None,
                             scores: torch.Tensor | None = None, out: torch.Tensor | None = None,
-                            err_flag: torch.Tensor | None = None) -> torch.Tensor:
+                            err_flag: torch.Tensor | None = None, prefix_final: bool = False) -> torch.Tensor:
     """GQA decode attention of streams that share a prefix (``kani_prefix_decode_attention``).
 
     One query token per stream attends to the prefix rows, which all streams share
@@ -1204,6 +1204,9 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
             heads of its KV head, is added to it (the running weight ``evict_cache``
             keeps by).
         out: optional contiguous output of B * Hq * D elements.
+        prefix_final: as in ``decode_attention``, for a decode step whose launch just
+            before writes at most q and each stream's newest row: the older rows and the
+            prefix stream in while it runs (``kani_prefix_decode_attention_step``).
     Returns out [B, Hq, D]; zeros where a stream sees no row at all.  A length out of
     range is held to it and flagged in ``err_flag``.
     """
@@ -1241,8 +1244,9 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
             raise ValueError(f"out must be a contiguous {q.dtype} tensor of {b * hq * d} elements")
         _refuse_overlap(((out, "out"),), inputs + ((scores, "scores"),))
     ws, n = _prefix_workspace(q.device, index, b, hq, hk, d, s_len, rows, scores is not None)
-    _call(index, "kani_prefix_decode_attention", lib.kani_prefix_decode_attention,
-          code, b, hq, hk, d, qv.data_ptr(), qb, qh, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
+    fn, name = ((lib.kani_prefix_decode_attention_step, "kani_prefix_decode_attention_step") if prefix_final
+                else (lib.kani_prefix_decode_attention, "kani_prefix_decode_attention"))
+    _call(index, name, fn, code, b, hq, hk, d, qv.data_ptr(), qb, qh, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
           s_len, kv_len.data_ptr(), pk.data_ptr() if rows else 0, pv.data_ptr() if rows else 0, ph, ps, rows,
           0 if plen is None else plen.data_ptr(), scale, scores_at, sb, sh, out.data_ptr(), hq * d, d,
           0 if ws is None else ws.data_ptr(), n, _flag_ptr(err_flag, q.device))

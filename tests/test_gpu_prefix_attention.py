@@ -107,6 +107,32 @@ def test_decode(case, dtype):
     assert int(flag) == 0
 
 
+@pytest.mark.parametrize("case", DECODE[4:12], ids=lambda c: "-".join(map(str, c[:7])))
+def test_step_launch_reads_the_newest_row_after_its_writer(case):
+    """As a decode step calls it: the launch just before writes q and each stream's newest
+    row (a KV write by this library), and the step's attention sees them; bit for bit the
+    plain call's result, weights included."""
+    b, hq, hk, d, p, plen, s, lens = case
+    g = torch.Generator().manual_seed(5)
+    dt = torch.bfloat16
+    q, k, v, pk, pv = (make(sh, g, dt).to(DEV) for sh in ((b, hq, d), (b, hk, s, d), (b, hk, s, d), (hk, p, d), (hk, p, d)))
+    used = torch.tensor([plen], device=DEV)
+    n = torch.tensor(lens, device=DEV)
+    slot = (n - 1).clamp_min(0)
+    scores = torch.zeros(b, hk, s, device=DEV)
+    for _ in range(20):
+        kn, vn = (make((b, hk, 1, d), g, dt).to(DEV) for _ in range(2))
+        k1, v1, s1, s2 = k.clone(), v.clone(), scores.clone(), scores.clone()
+        torch.cuda.synchronize()
+        K.kv_cache_write(kn, vn, k, v, slot)
+        got = K.prefix_decode_attention(q, k, v, n, pk, pv, used, scores=s1, prefix_final=True)
+        torch.cuda.synchronize()
+        K.kv_cache_write(kn, vn, k1, v1, slot)
+        torch.cuda.synchronize()
+        want = K.prefix_decode_attention(q, k1, v1, n, pk, pv, used, scores=s2)
+        assert torch.equal(got, want) and torch.equal(s1, s2) and torch.equal(k, k1)
+
+
 def test_decode_without_prefix_is_decode_attention():
     g = torch.Generator().manual_seed(3)
     q, k, v = make((6, 16, 64), g, torch.bfloat16), make((6, 8, 200, 64), g, torch.bfloat16), make((6, 8, 200, 64), g, torch.bfloat16)

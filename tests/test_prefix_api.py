@@ -36,7 +36,8 @@ ATTENTION = [(dict(batch=-1), BAD), (dict(hk=0), BAD), (dict(hq=5), BAD), (dict(
 
 @pytest.mark.parametrize("change,status", ATTENTION, ids=str)
 @pytest.mark.parametrize("name,base", [("kani_prefix_decode_attention", DECODE),
-                                       ("kani_prefix_prefill_attention", PREFILL)], ids=["decode", "prefill"])
+                                       ("kani_prefix_decode_attention_step", DECODE),
+                                       ("kani_prefix_prefill_attention", PREFILL)], ids=["decode", "step", "prefill"])
 def test_attention_refusals(name, base, change, status):
     assert call(name, base, **change) == status
 
