@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
         }
         tile_sum = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       };
-      bool move = m == -INFINITY && n > 0;
+      bool move = real && m == -INFINITY && n > 0;
       if (!__any_sync(0xffffffffu, move)) {
         if (ragged) weights(std::false_type{});
         else weights(std::true_type{});
