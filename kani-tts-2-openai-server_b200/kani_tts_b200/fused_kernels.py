@@ -28,7 +28,6 @@ the reference, all deliberate:
 """
 from __future__ import annotations
 
-import functools
 import math
 
 import torch
@@ -1076,6 +1075,28 @@ def _on_one_device(ref: torch.Tensor, what: str, named) -> int:
     return index
 
 
+_checked: dict = {}
+
+
+def _once(check, *args):
+    """check(*args), done once per signature: the checks of a call look at its tensors'
+    shapes, strides, types and devices (and plain numbers) alone, so a call with the
+    signature of one that passed takes what was found then (checks cost 10 us, the
+    signature 3).  Overlaps go by addresses and are looked at every time."""
+    try:
+        key = (check, *[a if a is None or type(a) is int else (a.shape, a.stride(), a.dtype, a.get_device())
+                        for a in args])
+    except AttributeError:       # not a tensor: the check says so
+        return check(*args)
+    found = _checked.get(key)
+    if found is None:
+        found = check(*args)
+        if len(_checked) >= 4096:
+            _checked.clear()
+        _checked[key] = found
+    return found
+
+
 def _call(index: int, name: str, fn, *args) -> None:
     """One C call on device `index`'s current stream, with that device as the current one."""
     if torch.cuda.current_device() == index:
@@ -1113,32 +1134,30 @@ def _refuse_overlap(outs, ins) -> None:
             raise ValueError(f"{w} must not be an expanded view")
 
 
-def _lengths(t: torch.Tensor, n: int, what: str) -> torch.Tensor:
+def _check_lengths(t: torch.Tensor, n: int, what: str) -> None:
     if t.dtype != torch.int64 or t.numel() != n:
         raise ValueError(f"{what} must be int64 with {n} element{'s' if n != 1 else ''}")
-    return t.contiguous()
 
 
-def _shared_prefix(prefix_k, prefix_v, prefix_len, q, hk: int, d: int):
-    """The prefix as (k, v, rows, head stride, row stride, length); no prefix: zero rows."""
+def _check_prefix(prefix_k, prefix_v, prefix_len, q, hk: int, d: int):
+    """The prefix's head stride, row stride and rows (none: zeros)."""
     if prefix_k is None or prefix_v is None:
         if prefix_k is not prefix_v or prefix_len is not None:
             raise ValueError("prefix_k and prefix_v must be given together, and prefix_len only with them")
-        return None, None, 0, 0, 0, None
-    if prefix_k.dim() == 4 and prefix_k.shape[0] == 1:
-        prefix_k = prefix_k[0]
-    if prefix_v.dim() == 4 and prefix_v.shape[0] == 1:
-        prefix_v = prefix_v[0]
-    if prefix_k.dim() != 3 or prefix_k.shape[0] != hk or prefix_k.shape[2] != d or prefix_v.shape != prefix_k.shape:
-        raise ValueError(f"prefix_k / prefix_v must both be [{hk}, rows, {d}], got {tuple(prefix_k.shape)} / "
-                         f"{tuple(prefix_v.shape)}")
+        return 0, 0, 0
+    for t in (prefix_k, prefix_v):
+        if t.dim() not in (3, 4) or (t.dim() == 4 and t.shape[0] != 1) or t.shape[-3] != hk or t.shape[-1] != d or \
+                t.shape[-2] != prefix_k.shape[-2]:
+            raise ValueError(f"prefix_k / prefix_v must both be [{hk}, rows, {d}], got {tuple(prefix_k.shape)} / "
+                             f"{tuple(prefix_v.shape)}")
     if prefix_k.dtype != q.dtype or prefix_v.dtype != q.dtype:
         raise TypeError("the prefix must have the dtype of q")
-    st = prefix_k.stride()
-    if st != prefix_v.stride() or st[2] != 1:
+    st = prefix_k.stride()[-3:]
+    if st != prefix_v.stride()[-3:] or st[2] != 1:
         raise ValueError("prefix_k and prefix_v need the same strides with a contiguous last dim")
-    plen = None if prefix_len is None else _lengths(prefix_len, 1, "prefix_len")
-    return prefix_k, prefix_v, prefix_k.shape[1], st[0], st[1], plen
+    if prefix_len is not None:
+        _check_lengths(prefix_len, 1, "prefix_len")
+    return st[0], st[1], prefix_k.shape[-2]
 
 
 def _own_cache(k_cache, v_cache, q):
@@ -1160,26 +1179,40 @@ def _attention_scale(scale, d: int) -> float:
     return scale
 
 
-@functools.lru_cache(maxsize=1024)
-def _prefix_workspace_bytes(device_index: int, *sizes: int) -> int:
-    with torch.cuda.device(device_index):      # the split depends on the device's SMs
-        return int(load_library().kani_prefix_decode_workspace(*sizes))
+def _address(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _prefix_workspace(device: torch.device, index: int, *sizes: int):
-    """A call's device scratch.  It comes from the caching allocator on the current
-    stream (inside a capture from the graph's own pool), so calls on other streams
-    and other graphs never share it."""
-    n = _prefix_workspace_bytes(index, *sizes)
-    return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
-
-
-def _flag_ptr(err_flag: torch.Tensor | None, device: torch.device) -> int:
-    if err_flag is None:
-        return error_flag(device).data_ptr()
-    if err_flag.dtype != torch.int32 or err_flag.numel() < 1:
+def _check_flag(err_flag) -> None:
+    if err_flag is not None and (err_flag.dtype != torch.int32 or err_flag.numel() < 1):
         raise ValueError("err_flag must be an int32 device tensor")
-    return err_flag.data_ptr()
+
+
+def _check_prefix_decode(q, k_cache, v_cache, kv_len, prefix_k, prefix_v, prefix_len, scores, out, err_flag):
+    index = _on_one_device(q, "q", ((k_cache, "k_cache"), (v_cache, "v_cache"), (kv_len, "kv_len"),
+                                    (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (prefix_len, "prefix_len"),
+                                    (scores, "scores"), (out, "out"), (err_flag, "err_flag")))
+    code = dtype_code(q, "q")
+    (b, hk, s_len, d), cs = _own_cache(k_cache, v_cache, q)
+    if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[1] != 1) or q.shape[0] != b or q.shape[-1] != d or \
+            (q.stride(-1) != 1 and q.numel()):
+        raise ValueError(f"q must be [{b}, heads, {d}] with a contiguous last dim")
+    hq = q.shape[-2]
+    if hk == 0 or hq % hk:
+        raise ValueError(f"{hq} query heads do not group over {hk} KV heads")
+    _check_lengths(kv_len, b, "kv_len")
+    ph, ps, rows = _check_prefix(prefix_k, prefix_v, prefix_len, q, hk, d)
+    sb = sh = 0
+    if scores is not None:
+        sb, sh, _ = _score_strides(scores, b, hk, s_len, "scores")
+    if out is not None and (out.numel() != b * hq * d or out.dtype != q.dtype or not out.is_contiguous()):
+        raise ValueError(f"out must be a contiguous {q.dtype} tensor of {b * hq * d} elements")
+    _check_flag(err_flag)
+    with torch.cuda.device(index):             # the split depends on the device's SMs
+        scratch = int(load_library().kani_prefix_decode_workspace(b, hq, hk, d, s_len, rows, int(scores is not None)))
+    expanded = 0 in q.stride() and q.numel() > 0
+    return (index, code, b, hq, hk, d, q.stride(0), q.stride(-2), cs[0], cs[1], cs[2], s_len, ph, ps, rows, sb, sh,
+            scratch, expanded)
 
 
 def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor,
@@ -1210,47 +1243,56 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     Returns out [B, Hq, D]; zeros where a stream sees no row at all.  A length out of
     range is held to it and flagged in ``err_flag``.
     """
-    index = _on_one_device(q, "q", ((k_cache, "k_cache"), (v_cache, "v_cache"), (kv_len, "kv_len"),
-                                    (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (prefix_len, "prefix_len"),
-                                    (scores, "scores"), (out, "out"), (err_flag, "err_flag")))
-    lib = load_library()
-    code = dtype_code(q, "q")
-    (b, hk, s_len, d), cs = _own_cache(k_cache, v_cache, q)
-    qv = q.squeeze(1) if q.dim() == 4 and q.shape[1] == 1 else q
-    if qv.dim() != 3 or qv.shape[0] != b or qv.shape[2] != d or (qv.stride(2) != 1 and qv.numel()):
-        raise ValueError(f"q must be [{b}, heads, {d}] with a contiguous last dim")
-    if 0 in qv.stride():
-        qv = qv.contiguous()        # (expanded over streams or heads)
-    qb, qh, _ = qv.stride()
-    hq = qv.shape[1]
-    if hk == 0 or hq % hk:
-        raise ValueError(f"{hq} query heads do not group over {hk} KV heads")
-    kv_len = _lengths(kv_len, b, "kv_len")
-    pk, pv, rows, ph, ps, plen = _shared_prefix(prefix_k, prefix_v, prefix_len, q, hk, d)
+    (index, code, b, hq, hk, d, qb, qh, cb, ch, cs, s_len, ph, ps, rows, sb, sh, scratch, expanded) = _once(
+        _check_prefix_decode, q, k_cache, v_cache, kv_len, prefix_k, prefix_v, prefix_len, scores, out, err_flag)
+    if expanded:                                # (over streams or heads)
+        q = q.contiguous()
+        qb, qh = hq * d, d
     scale = _attention_scale(scale, d)
-    sb = sh = scores_at = 0
-    inputs = ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (pk, "prefix_k"), (pv, "prefix_v"),
-              (kv_len, "kv_len"))
-    if scores is not None:
-        if scores.dtype != torch.float32 or scores.shape != (b, hk, s_len) or (scores.stride(2) != 1 and s_len > 1):
-            raise ValueError(f"scores must be fp32 [{b}, {hk}, {s_len}] with a contiguous last dim")
-        sb, sh, _ = scores.stride()
-        scores_at = scores.data_ptr()
-        _refuse_overlap(((scores, "scores"),), inputs)
+    if scores is not None or out is not None:
+        inputs = ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (prefix_k, "prefix_k"),
+                  (prefix_v, "prefix_v"), (kv_len, "kv_len"))
+        if scores is not None:
+            _refuse_overlap(((scores, "scores"),), inputs)
+        if out is not None:
+            _refuse_overlap(((out, "out"),), inputs + ((scores, "scores"),))
     if out is None:
         out = q.new_empty((b, hq, d))
-    else:
-        if out.numel() != b * hq * d or out.dtype != q.dtype or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {q.dtype} tensor of {b * hq * d} elements")
-        _refuse_overlap(((out, "out"),), inputs + ((scores, "scores"),))
-    ws, n = _prefix_workspace(q.device, index, b, hq, hk, d, s_len, rows, scores is not None)
+    # The call's scratch comes from the caching allocator on the current stream (inside a
+    # capture from the graph's own pool): calls on other streams and graphs never share it.
+    ws = torch.empty(scratch, dtype=torch.uint8, device=q.device) if scratch else None
+    kv_len = kv_len.contiguous()
+    lib = load_library()
     fn, name = ((lib.kani_prefix_decode_attention_step, "kani_prefix_decode_attention_step") if prefix_final
                 else (lib.kani_prefix_decode_attention, "kani_prefix_decode_attention"))
-    _call(index, name, fn, code, b, hq, hk, d, qv.data_ptr(), qb, qh, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
-          s_len, kv_len.data_ptr(), pk.data_ptr() if rows else 0, pv.data_ptr() if rows else 0, ph, ps, rows,
-          0 if plen is None else plen.data_ptr(), scale, scores_at, sb, sh, out.data_ptr(), hq * d, d,
-          0 if ws is None else ws.data_ptr(), n, _flag_ptr(err_flag, q.device))
+    _call(index, name, fn, code, b, hq, hk, d, q.data_ptr(), qb, qh, k_cache.data_ptr(), v_cache.data_ptr(), cb, ch,
+          cs, s_len, kv_len.data_ptr(), _address(prefix_k), _address(prefix_v), ph, ps, rows, _address(prefix_len),
+          scale, _address(scores), sb, sh, out.data_ptr(), hq * d, d, _address(ws), scratch,
+          (error_flag(q.device) if err_flag is None else err_flag).data_ptr())
     return out
+
+
+def _check_prefix_prefill(q, k_cache, v_cache, kv_len, prefix_k, prefix_v, prefix_len, q_len, out, err_flag):
+    index = _on_one_device(q, "q", ((k_cache, "k_cache"), (v_cache, "v_cache"), (kv_len, "kv_len"), (q_len, "q_len"),
+                                    (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (prefix_len, "prefix_len"),
+                                    (out, "out"), (err_flag, "err_flag")))
+    code = dtype_code(q, "q")
+    (b, hk, s_len, d), cs = _own_cache(k_cache, v_cache, q)
+    if q.dim() != 4 or q.shape[0] != b or q.shape[3] != d or (q.stride(3) != 1 and q.numel()):
+        raise ValueError(f"q must be [{b}, tokens, heads, {d}] with a contiguous last dim")
+    _, t, hq, _ = q.shape
+    if hk == 0 or hq % hk:
+        raise ValueError(f"{hq} query heads do not group over {hk} KV heads")
+    _check_lengths(kv_len, b, "kv_len")
+    if q_len is not None:
+        _check_lengths(q_len, b, "q_len")
+    ph, ps, rows = _check_prefix(prefix_k, prefix_v, prefix_len, q, hk, d)
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
+        raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)}")
+    _check_flag(err_flag)
+    qs = q.stride()
+    return (index, code, b, t, hq, hk, d, qs[0], qs[1], qs[2], cs[0], cs[1], cs[2], s_len, ph, ps, rows,
+            0 in qs and q.numel() > 0)
 
 
 def prefix_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor,
@@ -1274,38 +1316,55 @@ def prefix_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
             ``prefix_decode_attention``.  out: optional contiguous [B, T, Hq, D].
     Returns out [B, T, Hq, D].
     """
-    index = _on_one_device(q, "q", ((k_cache, "k_cache"), (v_cache, "v_cache"), (kv_len, "kv_len"), (q_len, "q_len"),
-                                    (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (prefix_len, "prefix_len"),
-                                    (out, "out"), (err_flag, "err_flag")))
-    lib = load_library()
-    code = dtype_code(q, "q")
-    (b, hk, s_len, d), cs = _own_cache(k_cache, v_cache, q)
-    if q.dim() != 4 or q.shape[0] != b or q.shape[3] != d or (q.stride(3) != 1 and q.numel()):
-        raise ValueError(f"q must be [{b}, tokens, heads, {d}] with a contiguous last dim")
-    _, t, hq, _ = q.shape
-    if hk == 0 or hq % hk:
-        raise ValueError(f"{hq} query heads do not group over {hk} KV heads")
-    kv_len = _lengths(kv_len, b, "kv_len")
-    q_len = None if q_len is None else _lengths(q_len, b, "q_len")
-    pk, pv, rows, ph, ps, plen = _shared_prefix(prefix_k, prefix_v, prefix_len, q, hk, d)
+    (index, code, b, t, hq, hk, d, qb, qt, qh, cb, ch, cs, s_len, ph, ps, rows, expanded) = _once(
+        _check_prefix_prefill, q, k_cache, v_cache, kv_len, prefix_k, prefix_v, prefix_len, q_len, out, err_flag)
+    if expanded:                                # (over streams, tokens or heads)
+        q = q.contiguous()
+        qb, qt, qh = t * hq * d, hq * d, d
     scale = _attention_scale(scale, d)
     if out is None:
         out = q.new_empty((b, t, hq, d))
     else:
-        if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)}")
-        _refuse_overlap(((out, "out"),), ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (pk, "prefix_k"),
-                                          (pv, "prefix_v"), (kv_len, "kv_len"), (q_len, "q_len")))
-    if 0 in q.stride():
-        q = q.contiguous()          # (expanded over streams, tokens or heads)
-    qs = q.stride()
-    _call(index, "kani_prefix_prefill_attention", lib.kani_prefix_prefill_attention,
-          code, b, t, hq, hk, d, q.data_ptr(), qs[0], qs[1], qs[2], k_cache.data_ptr(), v_cache.data_ptr(), cs[0],
-          cs[1], cs[2], s_len, kv_len.data_ptr(), 0 if q_len is None else q_len.data_ptr(),
-          pk.data_ptr() if rows else 0, pv.data_ptr() if rows else 0, ph, ps, rows,
-          0 if plen is None else plen.data_ptr(), scale, out.data_ptr(), t * hq * d, hq * d, d,
-          _flag_ptr(err_flag, q.device))
+        _refuse_overlap(((out, "out"),), ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"),
+                                          (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (kv_len, "kv_len"),
+                                          (q_len, "q_len")))
+    kv_len = kv_len.contiguous()
+    q_len = None if q_len is None else q_len.contiguous()
+    _call(index, "kani_prefix_prefill_attention", load_library().kani_prefix_prefill_attention,
+          code, b, t, hq, hk, d, q.data_ptr(), qb, qt, qh, k_cache.data_ptr(), v_cache.data_ptr(), cb, ch, cs, s_len,
+          kv_len.data_ptr(), _address(q_len), _address(prefix_k), _address(prefix_v), ph, ps, rows,
+          _address(prefix_len), scale, out.data_ptr(), t * hq * d, hq * d, d,
+          (error_flag(q.device) if err_flag is None else err_flag).data_ptr())
     return out
+
+
+def _check_evict(k_cache, v_cache, scores, kv_len, budget, recent, protect, k_out, v_out, scores_out, len_out, kept_out,
+                 err_flag):
+    index = _on_one_device(k_cache, "k_cache", ((v_cache, "v_cache"), (scores, "scores"), (kv_len, "kv_len"),
+                                                (k_out, "k_out"), (v_out, "v_out"), (scores_out, "scores_out"),
+                                                (len_out, "len_out"), (kept_out, "kept_out"), (err_flag, "err_flag")))
+    code = dtype_code(k_cache, "k_cache")
+    (b, hk, s_len, d), cs = _own_cache(k_cache, v_cache, k_cache)
+    ss = _score_strides(scores, b, hk, s_len, "scores")
+    _check_lengths(kv_len, b, "kv_len")
+    if (k_out is None) != (v_out is None) or (k_out is None) != (scores_out is None):
+        raise ValueError("k_out, v_out and scores_out must be given together (or none of them: in place)")
+    out_len, co, so = s_len, cs, ss
+    if k_out is not None:
+        (bo, hko, out_len, do), co = _own_cache(k_out, v_out, k_cache)
+        if (bo, hko, do) != (b, hk, d):
+            raise ValueError(f"k_out / v_out must be [{b}, {hk}, rows, {d}]")
+        so = _score_strides(scores_out, b, hk, out_len, "scores_out")
+    if budget < 0 or recent < 0 or protect < 0 or protect + recent > budget or budget > out_len:
+        raise ValueError(f"0 <= protect + recent <= budget <= {out_len} expected, got protect {protect}, "
+                         f"recent {recent}, budget {budget}")
+    if len_out is not None and (len_out.dtype != torch.int64 or len_out.numel() != b or not len_out.is_contiguous()):
+        raise ValueError(f"len_out must be contiguous int64 with {b} elements")
+    if kept_out is not None and (kept_out.dtype != torch.int32 or kept_out.shape != (b, hk, budget) or
+                                 not kept_out.is_contiguous()):
+        raise ValueError(f"kept_out must be contiguous int32 [{b}, {hk}, {budget}]")
+    _check_flag(err_flag)
+    return (index, code, b, hk, d, cs[0], cs[1], cs[2], s_len, ss[0], ss[1], co[0], co[1], co[2], out_len, so[0], so[1])
 
 
 def evict_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor, kv_len: torch.Tensor, budget: int,
@@ -1334,50 +1393,30 @@ def evict_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tens
     length become zero (the next rows start from there); K / V rows past it stay as
     they were.
     """
-    index = _on_one_device(k_cache, "k_cache", ((v_cache, "v_cache"), (scores, "scores"), (kv_len, "kv_len"),
-                                                (k_out, "k_out"), (v_out, "v_out"), (scores_out, "scores_out"),
-                                                (len_out, "len_out"), (kept_out, "kept_out"), (err_flag, "err_flag")))
-    lib = load_library()
-    code = dtype_code(k_cache, "k_cache")
-    (b, hk, s_len, d), cs = _own_cache(k_cache, v_cache, k_cache)
-    ss = _score_strides(scores, b, hk, s_len, "scores")
-    kv_len = _lengths(kv_len, b, "kv_len")
-    if (k_out is None) != (v_out is None) or (k_out is None) != (scores_out is None):
-        raise ValueError("k_out, v_out and scores_out must be given together (or none of them: in place)")
+    budget, recent, protect = int(budget), int(recent), int(protect)
+    (index, code, b, hk, d, cb, ch, cs, s_len, sb, sh, ob, oh, os_, out_len, sob, soh) = _once(
+        _check_evict, k_cache, v_cache, scores, kv_len, budget, recent, protect, k_out, v_out, scores_out, len_out,
+        kept_out, err_flag)
     inputs = ((kv_len, "kv_len"),)
     if k_out is not None:
-        (bo, hko, out_len, do), co = _own_cache(k_out, v_out, k_cache)
-        if (bo, hko, do) != (b, hk, d):
-            raise ValueError(f"k_out / v_out must be [{b}, {hk}, rows, {d}]")
-        so = _score_strides(scores_out, b, hk, out_len, "scores_out")
         inputs = ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores"), (kv_len, "kv_len"))
     else:
-        k_out, v_out, scores_out, out_len, co, so = k_cache, v_cache, scores, s_len, cs, ss
+        k_out, v_out, scores_out = k_cache, v_cache, scores
+        if len_out is not None or kept_out is not None:
+            _refuse_overlap(((len_out, "len_out"), (kept_out, "kept_out")),
+                            ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores")))
     if k_out.data_ptr() == v_out.data_ptr() and k_out.numel():
         raise ValueError("keys and values must be different tensors")
-    budget, recent, protect = int(budget), int(recent), int(protect)
-    if budget < 0 or recent < 0 or protect < 0 or protect + recent > budget or budget > out_len:
-        raise ValueError(f"0 <= protect + recent <= budget <= {out_len} expected, got protect {protect}, "
-                         f"recent {recent}, budget {budget}")
-    if len_out is not None and (len_out.dtype != torch.int64 or len_out.numel() != b or not len_out.is_contiguous()):
-        raise ValueError(f"len_out must be contiguous int64 with {b} elements")
-    kept_at = 0
-    if kept_out is not None:
-        if kept_out.dtype != torch.int32 or kept_out.shape != (b, hk, budget) or not kept_out.is_contiguous():
-            raise ValueError(f"kept_out must be contiguous int32 [{b}, {hk}, {budget}]")
-        kept_at = kept_out.data_ptr()
     _refuse_overlap(((k_out, "k_out"), (v_out, "v_out"), (scores_out, "scores_out"), (len_out, "len_out"),
                      (kept_out, "kept_out")), inputs)
-    if k_out is k_cache and (len_out is not None or kept_out is not None):
-        _refuse_overlap(((len_out, "len_out"), (kept_out, "kept_out")),
-                        ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores")))
     if len_out is None:
         len_out = kv_len.new_empty(b)
-    _call(index, "kani_cache_evict", lib.kani_cache_evict,
-          code, b, hk, d, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], s_len, scores.data_ptr(),
-          ss[0], ss[1], kv_len.data_ptr(), budget, recent, protect, k_out.data_ptr(), v_out.data_ptr(), co[0], co[1],
-          co[2], out_len, scores_out.data_ptr(), so[0], so[1], len_out.data_ptr(), kept_at,
-          _flag_ptr(err_flag, k_cache.device))
+    kv_len = kv_len.contiguous()
+    _call(index, "kani_cache_evict", load_library().kani_cache_evict,
+          code, b, hk, d, k_cache.data_ptr(), v_cache.data_ptr(), cb, ch, cs, s_len, scores.data_ptr(), sb, sh,
+          kv_len.data_ptr(), budget, recent, protect, k_out.data_ptr(), v_out.data_ptr(), ob, oh, os_, out_len,
+          scores_out.data_ptr(), sob, soh, len_out.data_ptr(), _address(kept_out),
+          (error_flag(k_cache.device) if err_flag is None else err_flag).data_ptr())
     return len_out
 
 
