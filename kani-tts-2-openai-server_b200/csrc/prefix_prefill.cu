@@ -391,10 +391,13 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
         }
       };
       // The weights relative to the maximum so far, without looking for a new one: a
-      // sum that passes 2^10 (or a first look at the row) shows that it is needed.
+      // sum that passes 2^10 (or a first look at the row) shows that it is needed.  Only
+      // such rows move, so a row's result does not depend on the others of its warp.
       uint32_t pk[32];
       float tile_sum = 0.f;
-      auto weights = [&](auto mixed) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) pk[i] = 0u;
+      auto weights = [&](auto mixed, bool want) {
         const float ms = m == -INFINITY ? 0.f : m;
         const float2 c2 = make_float2(p.qscale, p.qscale), m2 = make_float2(-ms, -ms);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -409,15 +412,16 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
           else
             w = make_float2(ex2(x.x), ex2(x.y));
           sum[i & 1] = __fadd2_rn(sum[i & 1], w);
-          pk[i] = pack2<T>(w.x, w.y);
+          const uint32_t both = pack2<T>(w.x, w.y);
+          pk[i] = want ? both : pk[i];
         }
-        tile_sum = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        tile_sum = want ? (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y) : tile_sum;
       };
-      bool move = real && m == -INFINITY && n > 0;
-      if (!__any_sync(0xffffffffu, move)) {
-        if (ragged) weights(std::false_type{});
-        else weights(std::true_type{});
-        move = tile_sum > kMaxSum;
+      bool move = real && m == -INFINITY && n > 0;  // a first look
+      if (!__all_sync(0xffffffffu, move || !real)) {
+        if (ragged) weights(std::false_type{}, true);
+        else weights(std::true_type{}, true);
+        move = move || (real && tile_sum > kMaxSum);
       }
       if (__any_sync(0xffffffffu, move)) {
         float mx = -INFINITY;
@@ -427,7 +431,7 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
 #pragma unroll
           for (int i = 0; i < 64; i += 2) mx = max3(mx, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
         }
-        const float mn = fmaxf(m, mx * p.qscale), w = merge_weight(m, mn);
+        const float mn = move ? fmaxf(m, mx * p.qscale) : m, w = move ? merge_weight(m, mn) : 1.f;
         if (j > 0) {
           if (!wait_all(bars.pv, (uint32_t)((j - 1) & 1))) break;
           tc::fence_after_sync();
@@ -443,7 +447,7 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
           }
         }
         m = mn;
-        weights(std::false_type{});
+        weights(std::false_type{}, move);
       }
       l += tile_sum;
       tmem_st32(sp, pk);  // over S, which has been read

@@ -70,6 +70,13 @@ DECODE = [
     (130, 2, 1, 64, 1025, 1000, 33, [(i * 7) % 34 for i in range(130)]),
     (3, 4, 2, 64, 33, 0, 2100, [2100, 2049, 0]),
     (2, 4, 4, 128, 9, 9, 1500, [1500, 1023]),
+    (3, 8, 1, 64, 0, 0, 40000, [40000, 39999, 1]),          # logits in the workspace
+    # from 128 MB of prefix rows times streams on: the prefix in a launch of its own
+    (130, 16, 2, 64, 2100, 2000, 33, [(i * 7) % 34 for i in range(130)]),
+    (70, 8, 2, 128, 2000, 2000, 40, [(i * 11) % 41 for i in range(70)]),
+    (100, 14, 2, 64, 2700, 2689, 17, [(i * 5) % 18 for i in range(100)]),
+    (8, 3, 1, 64, 70000, 69937, 200, [0, 1, 200, 64, 63, 130, 7, 0]),      # several partial results
+    (300, 2, 1, 64, 1800, 0, 5, [i % 6 for i in range(300)]),              # a prefix of which nothing is used
 ]
 
 
@@ -107,7 +114,7 @@ def test_decode(case, dtype):
     assert int(flag) == 0
 
 
-@pytest.mark.parametrize("case", DECODE[4:12], ids=lambda c: "-".join(map(str, c[:7])))
+@pytest.mark.parametrize("case", DECODE[4:12] + DECODE[14:18], ids=lambda c: "-".join(map(str, c[:7])))
 def test_step_launch_reads_the_newest_row_after_its_writer(case):
     """As a decode step calls it: the launch just before writes q and each stream's newest
     row (a KV write by this library), and the step's attention sees them; bit for bit the
@@ -371,7 +378,7 @@ def test_captured_graphs_and_other_streams():
     for the inputs of the replay, and scores add up once per replay."""
     g = torch.Generator().manual_seed(41)
     dt = torch.bfloat16
-    b, hq, hk, d, p, s = 24, 16, 8, 64, 600, 300
+    b, hq, hk, d, p, s = 24, 16, 8, 64, 2800, 300      # (over 128 MB: two launches)
     sets = []
     for _ in range(2):
         x = [make(sh, g, dt).to(DEV) for sh in ((b, hq, d), (b, hk, s, d), (b, hk, s, d), (hk, p, d), (hk, p, d))]
@@ -413,6 +420,25 @@ def test_captured_graphs_and_other_streams():
     torch.cuda.synchronize()
     x, n, _ = sets[0]
     assert torch.equal(outs[0][0], K.prefix_decode_attention(x[0], x[1], x[2], n, x[3], x[4], scores=torch.zeros(b, hk, s, device=DEV)))
+
+
+def test_two_streams_at_once():
+    """The same call on two streams, interleaved: every result is the one alone."""
+    g = torch.Generator().manual_seed(43)
+    q, k, v, pk, pv = (make(sh, g, torch.bfloat16).to(DEV) for sh in ((64, 16, 64), (64, 8, 300, 64), (64, 8, 300, 64),
+                                                                     (8, 2048, 64), (8, 2048, 64)))
+    n = torch.randint(0, 301, (64,), generator=g).to(DEV)
+    want = K.prefix_decode_attention(q, k, v, n, pk, pv)
+    pre = K.prefix_prefill_attention(q[:, None].expand(64, 7, 16, 64), k, v, n.clamp_min(7), pk, pv)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in range(20):
+        for st in streams:
+            with torch.cuda.stream(st):
+                outs.append((K.prefix_decode_attention(q, k, v, n, pk, pv),
+                             K.prefix_prefill_attention(q[:, None].expand(64, 7, 16, 64), k, v, n.clamp_min(7), pk, pv)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want) and torch.equal(b, pre) for a, b in outs)
 
 
 def test_offsets_past_32_bits():
