@@ -12,6 +12,7 @@
 // Moving the kept rows bounds it.  A cluster of 1, 2, 4 or 8 CTAs works on one
 // (b, h): every CTA finds the kept rows for itself and moves its share of the columns
 // of the rows [K | V], so in-place moves of different CTAs never meet.
+// (Out of place, further clusters may share the rows of long caches.)
 //   * Selection: the scores' bits in an order where unsigned comparison is theirs; the
 //     most-th largest by radix selection over digits of 11, 11 and 10 bits, with a
 //     histogram in shared memory; ties beyond it go by slot.  Counts are integers, so

@@ -57,7 +57,8 @@ template <int D> struct FlashShape {
   static constexpr int kStages = D == 64 ? 4 : 2;
   // One pair of weights in so many by polynomial instead of the special-function unit,
   // which takes 8 cycles for a warp's 32: with D = 64 that unit is the busiest (4 x 4096
-  // tokens behind 4096 rows: none 610 us, one in 4 565, one in 6 552, one in 8 557), with
+  // tokens behind 4096 rows: none 610 us, one in 4 565, one in 6 552, one in 8 557 before
+  // rows moved their maxima alone, 560 with it), with
   // D = 128 the products weigh twice as much (3 x 777 tokens: none 55.7 us, one in 4 58.0).
   static constexpr int kFmaOneIn = D == 64 ? 6 : 0;
   static constexpr uint32_t kQBytes = kRows * D * 2;
@@ -395,9 +396,7 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
       // such rows move, so a row's result does not depend on the others of its warp.
       uint32_t pk[32];
       float tile_sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) pk[i] = 0u;
-      auto weights = [&](auto mixed, bool want) {
+      auto weights = [&](auto mixed, auto always, bool want) {
         const float ms = m == -INFINITY ? 0.f : m;
         const float2 c2 = make_float2(p.qscale, p.qscale), m2 = make_float2(-ms, -ms);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -413,15 +412,18 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
             w = make_float2(ex2(x.x), ex2(x.y));
           sum[i & 1] = __fadd2_rn(sum[i & 1], w);
           const uint32_t both = pack2<T>(w.x, w.y);
-          pk[i] = want ? both : pk[i];
+          pk[i] = decltype(always)::value || want ? both : pk[i];
         }
-        tile_sum = want ? (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y) : tile_sum;
+        if (decltype(always)::value || want) tile_sum = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       };
-      bool move = real && m == -INFINITY && n > 0;  // a first look
-      if (!__all_sync(0xffffffffu, move || !real)) {
-        if (ragged) weights(std::false_type{}, true);
-        else weights(std::true_type{}, true);
-        move = move || (real && tile_sum > kMaxSum);
+      // (in a tile that some row has its first look at, the rows that do not either see
+      // nothing or, the tile being ragged, take the same weights here as below)
+      bool move = real && m == -INFINITY && n > 0;
+      const bool look = __any_sync(0xffffffffu, move);
+      if (!look) {
+        if (ragged) weights(std::false_type{}, std::true_type{}, true);
+        else weights(std::true_type{}, std::true_type{}, true);
+        move = real && tile_sum > kMaxSum;
       }
       if (__any_sync(0xffffffffu, move)) {
         float mx = -INFINITY;
@@ -447,7 +449,7 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
           }
         }
         m = mn;
-        weights(std::false_type{}, move);
+        weights(std::false_type{}, std::false_type{}, look || move);
       }
       l += tile_sum;
       tmem_st32(sp, pk);  // over S, which has been read
