@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
     const int all = min(own, start + t0 + 1);              // own rows that every real row sees
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
     float m = -INFINITY, l = 0.f;
-    bool ok = true;
+    bool ok = true, live = real;  // live: the row's maximum may still move
     auto wait_all = [&](const uint64_t& x, uint32_t parity) {  // the same answer in all lanes
       return ok = __all_sync(0xffffffffu, tc::wait(bar(x), parity));
     };
@@ -392,8 +392,8 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
         }
       };
       // The weights relative to the maximum so far, without looking for a new one: a
-      // sum that passes 2^10 (or a first look at the row) shows that it is needed.  Only
-      // such rows move, so a row's result does not depend on the others of its warp.
+      // sum that passes 2^10 (or a row that has no maximum yet) shows that it is needed.
+      // Only such rows move, so a row's result does not depend on the others of its warp.
       uint32_t pk[32];
       float tile_sum = 0.f;
       auto weights = [&](auto mixed, auto always, bool want) {
@@ -416,14 +416,16 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
         }
         if (decltype(always)::value || want) tile_sum = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       };
-      // (in a tile that some row has its first look at, the rows that do not either see
-      // nothing or, the tile being ragged, take the same weights here as below)
-      bool move = real && m == -INFINITY && n > 0;
-      const bool look = __any_sync(0xffffffffu, move);
-      if (!look) {
+      // A row whose logits have all been -inf asks again in every tile, one that has met a
+      // NaN does not.  The rows beside it are served as ever: the pass is left out only
+      // where no row has a maximum to go by, as in the first tile.
+      bool move = live && m == -INFINITY && n > 0;
+      bool pass = !__any_sync(0xffffffffu, move);
+      if (!pass) pass = __any_sync(0xffffffffu, m != -INFINITY);
+      if (pass) {
         if (ragged) weights(std::false_type{}, std::true_type{}, true);
         else weights(std::true_type{}, std::true_type{}, true);
-        move = real && tile_sum > kMaxSum;
+        move = move || (live && tile_sum > kMaxSum);
       }
       if (__any_sync(0xffffffffu, move)) {
         float mx = -INFINITY;
@@ -449,7 +451,8 @@ __global__ void __launch_bounds__(kFlashThreads, 2) prefix_flash_kernel(const __
           }
         }
         m = mn;
-        weights(std::false_type{}, std::false_type{}, look || move);
+        weights(std::false_type{}, std::false_type{}, !pass || move);
+        live = live && tile_sum == tile_sum;
       }
       l += tile_sum;
       tmem_st32(sp, pk);  // over S, which has been read
