@@ -681,6 +681,9 @@ class DecodeEngine:
     ``cache_recent`` rows (default: half of what the prompt leaves of the budget) and
     the rows with the most accumulated attention weight.  The shared prefix of
     ``FusedDecoder.set_prefix`` is never cut.
+
+    A captured step serves every later ``start`` of at most the ``max_new_tokens`` that it
+    was captured with; ``generated`` is a tensor of each start's own.
     """
 
     def __init__(self, decoder: FusedDecoder, keep_mask: bool = False, sampling: SamplingParams | None = None,
@@ -697,6 +700,8 @@ class DecodeEngine:
         self._filled = 0                 # own rows in the caches (every stream's)
         self._prompt_rows = 0
         self._captured_prefix = None
+        self._tokens = None              # where the captured step writes its tokens
+        self._steps = 0                  # steps since start
         self.keep_mask = keep_mask   # maintain the additive mask (for steps that use one)
         self.sampling = sampling
         dev, b, s = decoder.device, decoder.batch, decoder.max_len
@@ -740,7 +745,11 @@ class DecodeEngine:
         self.rng_step.zero_()
         if self.sampling is not None:
             # the prompt is the initial repetition history (inference_engine.py:553-556)
-            self.seen = seen_bitmap(history, dec.head.shape[0], dec.full_to_reduced, device=dec.device)
+            seen = seen_bitmap(history, dec.head.shape[0], dec.full_to_reduced, device=dec.device)
+            if self.seen is None:
+                self.seen = seen
+            else:
+                self.seen.copy_(seen)     # a captured step goes on from this memory
         first = self._next_token(logits[:, -1])
         self.rng_step.add_(1)
         self.input_ids.copy_(first.view(b, 1))
@@ -754,15 +763,18 @@ class DecodeEngine:
         self.kv_len.copy_(self.base_slot + 1)
         self.generated = torch.zeros(b, max_new_tokens, dtype=torch.long, device=dec.device)
         self._filled = self._prompt_rows = t_eff
+        self._steps = 0
 
-    def _step_body(self):
+    def _step_body(self, tokens: torch.Tensor | None = None):
+        """One step, its token into `tokens` (default: ``generated``, as a step of the loop)."""
         self.dec.scores = self.scores    # for this engine's steps alone
         try:
-            self._step_launches()
+            self._step_launches(self.generated if tokens is None else tokens)
         finally:
             self.dec.scores = None
+        self._steps += tokens is None
 
-    def _step_launches(self):
+    def _step_launches(self, tokens: torch.Tensor):
         cfg = self.dec.cfg
         if self.keep_mask:
             self.mask.scatter_(3, self.slots.view(-1, 1, 1, 1), 0.0)
@@ -776,7 +788,7 @@ class DecodeEngine:
             self.logits = self.dec.step(self.input_ids, self.positions, self.slots, self.kv_len, self.mask)
             nxt = self._next_token(self.logits[:, 0])
         # record and feed back the token, next step's position / slot / length, counters
-        decode_advance(nxt.view(-1), self.input_ids, self.generated, self.step_idx, self.base_pos, self.base_slot,
+        decode_advance(nxt.view(-1), self.input_ids, tokens, self.step_idx, self.base_pos, self.base_slot,
                        self.positions, self.slots, self.kv_len, cfg.tokens_per_frame, cfg.audio_step,
                        rng_step=self.rng_step if self.sampling is not None else None)
 
@@ -792,8 +804,11 @@ class DecodeEngine:
         return self.next_tok
 
     def capture(self) -> None:
-        """Warm up once outside capture, then capture one decode step."""
+        """Warm up once outside capture, then capture one decode step.  It keeps the
+        addresses of what it reads and writes: the engine's own buffers, which later starts
+        refill, and a token buffer that `run` copies from."""
         dec = self.dec
+        tokens = torch.zeros_like(self.generated)
         saved = ({i: c.clone() for i, c in dec.conv_state.items()}, self.input_ids.clone(), self.mask.clone(),
                  self.step_idx.clone(), self.rng_step.clone(),
                  self.seen.clone() if self.seen is not None else None,
@@ -802,11 +817,11 @@ class DecodeEngine:
         s = torch.cuda.Stream(device=dec.device)
         s.wait_stream(torch.cuda.current_stream(dec.device))
         with torch.cuda.stream(s):
-            self._step_body()
+            self._step_body(tokens)
         torch.cuda.current_stream(dec.device).wait_stream(s)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
-            self._step_body()
+            self._step_body(tokens)
         # undo the warm-up and capture steps (they ran the step twice)
         for i, c in saved[0].items():
             dec.conv_state[i].copy_(c)
@@ -821,7 +836,7 @@ class DecodeEngine:
         self.kv_len.copy_(saved[8])
         for i, t in saved[9].items():
             self.scores[i].copy_(t)
-        self._captured_prefix = dec.prefix   # the graph reads its buffers
+        self._captured_prefix, self._tokens = dec.prefix, tokens   # the graph's buffers
 
     def _evict(self) -> None:
         """Cut the full caches down to the budget; the next step writes behind what is left."""
@@ -836,8 +851,14 @@ class DecodeEngine:
     def run(self, n_steps: int) -> None:
         if self.dec.prefix is not self._captured_prefix:
             raise RuntimeError("the shared prefix's buffers are not those of the captured step: capture() again")
+        if self._tokens is None or self.generated.shape[1] > self._tokens.shape[1]:
+            raise RuntimeError("no step has been captured for this many new tokens: capture() again")
         for _ in range(n_steps):
             if self.cache_budget is not None and self._filled == self.dec.max_len:
                 self._evict()
             self.graph.replay()
             self._filled += 1
+        new = slice(self._steps, min(self._steps + n_steps, self.generated.shape[1]))
+        if new.start < new.stop:
+            self.generated[:, new].copy_(self._tokens[:, new])
+        self._steps += n_steps
