@@ -728,9 +728,10 @@ class DecodeEngine:
         if self.cache_budget is None:
             if t_eff + max_new_tokens > dec.max_len:
                 raise ValueError(f"cache of {dec.max_len} slots cannot hold {t_eff} + {max_new_tokens} tokens")
-        elif t_eff + (self.cache_recent or 0) > self.cache_budget:
-            raise ValueError(f"a prompt of {t_eff} rows and {self.cache_recent or 0} recent ones do not fit a budget "
-                             f"of {self.cache_budget}")
+        elif t_eff + max(self.cache_recent or 0, 1) > self.cache_budget:
+            # (the prompt's rows always stay: without room behind them an eviction drops all others)
+            raise ValueError(f"a prompt of {t_eff} rows and {max(self.cache_recent or 0, 1)} recent ones do not fit a "
+                             f"budget of {self.cache_budget}")
         history, before = input_ids, 0
         if dec.prefix is None:
             pos = _prompt_positions(cfg, input_ids, t_eff, speaker_emb is not None)
