@@ -565,6 +565,8 @@ class FusedDecoder:
         Returns P', the prefix's rows.
         """
         cfg, dev = self.cfg, self.device
+        if input_ids.dim() not in (1, 2) or (input_ids.dim() == 2 and input_ids.shape[0] != 1):
+            raise ValueError(f"a prefix is one sequence [P] or [1, P], got {tuple(input_ids.shape)}")
         ids = input_ids.reshape(1, -1).to(dev)
         if ids.shape[1] == 0:
             raise ValueError("an empty prefix: use clear_prefix")
