@@ -573,6 +573,8 @@ class FusedDecoder:
         rows = ids.shape[1] + (speaker_emb is not None)
         if positions is None:
             positions = _prompt_positions(cfg, ids, rows, speaker_emb is not None)
+        elif positions.numel() != rows:
+            raise ValueError(f"positions must be [1, {rows}], got {tuple(positions.shape)}")
         p = self.prefix
         if p is None or rows > p.capacity or (capacity or 0) > p.capacity:
             cap = max(rows, capacity or 0)

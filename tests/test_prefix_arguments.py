@@ -34,3 +34,16 @@ def test_several_sequences_are_not_run_together(shape):
     """One prefix serves all streams: a batch of prompts is not their concatenation."""
     with pytest.raises(ValueError):
         FusedDecoder.set_prefix(decoder(), torch.ones(shape, dtype=torch.long))
+
+
+@pytest.mark.parametrize("speaker", [False, True])
+def test_positions_of_another_length_are_refused(speaker):
+    """Before the pass: it fills the buffers of a prefix that may be in use layer by layer."""
+    spk = torch.zeros(1, 32) if speaker else None
+    for n in (8, 10, 11):
+        if n == 9 + speaker:
+            continue
+        with pytest.raises(ValueError):
+            FusedDecoder.set_prefix(decoder(), torch.ones(9, dtype=torch.long), torch.arange(n).view(1, n), spk)
+    with pytest.raises(Pass):
+        FusedDecoder.set_prefix(decoder(), torch.ones(9, dtype=torch.long), torch.arange(9 + speaker).view(1, -1), spk)
