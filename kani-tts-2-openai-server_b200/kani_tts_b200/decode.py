@@ -813,6 +813,8 @@ class DecodeEngine:
         addresses of what it reads and writes: the engine's own buffers, which later starts
         refill, and a token buffer that `run` copies from."""
         dec = self.dec
+        if self.cache_budget is not None and self._filled == dec.max_len:
+            self._evict()                # the warm-up step takes a row
         tokens = torch.zeros_like(self.generated)
         saved = ({i: c.clone() for i, c in dec.conv_state.items()}, self.input_ids.clone(), self.mask.clone(),
                  self.step_idx.clone(), self.rng_step.clone(),

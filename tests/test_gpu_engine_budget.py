@@ -64,3 +64,29 @@ def test_tokens_before_an_eviction_are_the_plain_engines(b, with_prefix):
         assert torch.equal(tokens[30][sure, i], tokens[None][sure, i])
         clear += int(sure.sum())
     assert clear > 0
+
+
+def test_a_capture_when_the_caches_are_full():
+    """The warm-up step of a capture needs a row too: captured again with full caches, the
+    engine goes on as one that was not, and no slot past the end is written."""
+    cfg = tiny_config()
+    sd = synthetic_state_dict(cfg, seed=9)
+    own = torch.randint(10, cfg.audio_tokens_start, (2, 6), generator=torch.Generator().manual_seed(8)).to(DEV)
+    results = []
+    for again in (False, True):
+        dec = FusedDecoder(cfg, sd, DEV, batch=2, max_len=20)
+        eng = DecodeEngine(dec, cache_budget=12, cache_recent=3)
+        eng.start(own, None, 40)
+        eng.capture()
+        eng.run(14)
+        assert eng._filled == 20
+        if again:
+            eng.capture()
+        eng.run(26)
+        torch.cuda.synchronize()
+        assert int(dec.err_flag.item()) == 0
+        results.append((eng.generated.clone(), eng.positions.clone(), eng.kv_len.clone(),
+                        *(t.clone() for t in eng.scores.values())))
+        eng.graph = None
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
