@@ -1119,19 +1119,49 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
     return first, first + (last + 1) * t.element_size()
 
 
-def _refuse_overlap(outs, ins) -> None:
+def _refuse_overlap(outs, ins, then=()) -> None:
     """Outputs that a call writes while it still reads its inputs must lie apart from
-    them, and may not be expanded views.  Both: (tensor or None, name) pairs."""
+    them, and those of `then` also from the outputs before them.  All: (tensor or None,
+    name) pairs."""
     spans = [(*_span(t), w) for t, w in ins if t is not None]
-    for t, w in outs:
-        if t is None:
-            continue
-        a0, a1 = _span(t)
-        for b0, b1, other in spans:
-            if a0 < b1 and b0 < a1:
-                raise ValueError(f"{w} must not overlap {other}")
-        if 0 in t.stride() and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
-            raise ValueError(f"{w} must not be an expanded view")
+    inputs = len(spans)
+    for group, first in ((outs, True), (then, False)):
+        for t, w in group:
+            if t is None:
+                continue
+            a0, a1 = _span(t)
+            for b0, b1, other in spans[:inputs] if first else spans:
+                if a0 < b1 and b0 < a1:
+                    raise ValueError(f"{w} must not overlap {other}")
+            spans.append((a0, a1, w))
+
+
+def _refuse_strides(dims, message: str) -> None:
+    """(stride, size) pairs under which two elements may have one address: sorted, each
+    stride has to pass the elements below it."""
+    past = 1
+    for st, n in sorted(dims):
+        if n > 1:
+            if st < past:
+                raise ValueError(message)
+            past += (n - 1) * st
+
+
+def _refuse_shared(t: torch.Tensor, what: str) -> None:
+    """An output's elements must lie apart: no expanded view, no overlapping windows."""
+    if t.numel():
+        _refuse_strides(zip(t.stride(), t.shape), f"{what} must not be an expanded or overlapping view")
+
+
+def _refuse_shared_rows(k: torch.Tensor, v: torch.Tensor) -> None:
+    """Keys and values that a call writes, of equal shapes and strides, must lie apart;
+    their rows may alternate in one buffer."""
+    apart = abs(v.data_ptr() - k.data_ptr())
+    if k.numel() and not (k.is_contiguous() and apart >= k.nbytes):
+        es = k.element_size()
+        if apart % es:
+            raise ValueError("keys and values must not overlap")
+        _refuse_strides([*zip(k.stride(), k.shape), (apart // es, 2)], "keys and values must not overlap")
 
 
 def _check_lengths(t: torch.Tensor, n: int, what: str) -> None:
@@ -1205,6 +1235,7 @@ def _check_prefix_decode(q, k_cache, v_cache, kv_len, prefix_k, prefix_v, prefix
     sb = sh = 0
     if scores is not None:
         sb, sh, _ = _score_strides(scores, b, hk, s_len, "scores")
+        _refuse_shared(scores, "scores")
     if out is not None and (out.numel() != b * hq * d or out.dtype != q.dtype or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous {q.dtype} tensor of {b * hq * d} elements")
     _check_flag(err_flag)
@@ -1355,6 +1386,9 @@ def _check_evict(k_cache, v_cache, scores, kv_len, budget, recent, protect, k_ou
         if (bo, hko, do) != (b, hk, d):
             raise ValueError(f"k_out / v_out must be [{b}, {hk}, rows, {d}]")
         so = _score_strides(scores_out, b, hk, out_len, "scores_out")
+    for t, w in ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores")) if k_out is None else (
+            (k_out, "k_out"), (v_out, "v_out"), (scores_out, "scores_out")):
+        _refuse_shared(t, w)
     if budget < 0 or recent < 0 or protect < 0 or protect + recent > budget or budget > out_len:
         raise ValueError(f"0 <= protect + recent <= budget <= {out_len} expected, got protect {protect}, "
                          f"recent {recent}, budget {budget}")
@@ -1402,13 +1436,9 @@ def evict_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tens
         inputs = ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores"), (kv_len, "kv_len"))
     else:
         k_out, v_out, scores_out = k_cache, v_cache, scores
-        if len_out is not None or kept_out is not None:
-            _refuse_overlap(((len_out, "len_out"), (kept_out, "kept_out")),
-                            ((k_cache, "k_cache"), (v_cache, "v_cache"), (scores, "scores")))
-    if k_out.data_ptr() == v_out.data_ptr() and k_out.numel():
-        raise ValueError("keys and values must be different tensors")
-    _refuse_overlap(((k_out, "k_out"), (v_out, "v_out"), (scores_out, "scores_out"), (len_out, "len_out"),
-                     (kept_out, "kept_out")), inputs)
+    _refuse_shared_rows(k_out, v_out)
+    _refuse_overlap(((k_out, "k_out"), (v_out, "v_out"), (scores_out, "scores_out")), inputs,
+                    ((len_out, "len_out"), (kept_out, "kept_out")))
     if len_out is None:
         len_out = kv_len.new_empty(b)
     kv_len = kv_len.contiguous()
