@@ -524,7 +524,11 @@ KANI_API int kani_codec_codes(const int64_t* tokens, int64_t tokens_row_stride, 
  *   out[b, hq, :] = sum_j w_j v_j,  w = softmax_j(scale * q[b, hq, :] . k_j),
  * j over prefix rows [0, *prefix_len) (prefix_len NULL: all prefix_rows) and own
  * rows [0, kv_len[b]); a query without any row gets zeros.  kani_decode_attention's
- * operation when prefix_rows is 0.  The prefix is read once for the whole batch.
+ * operation when prefix_rows is 0.  From 128 MiB of prefix K and V bytes times batch on,
+ * the prefix is read once for the whole batch, on the tensor cores, with its weights
+ * rounded to dtype before they meet the values; below, every stream's blocks read it (from
+ * L2 after the first) and keep 16 bits of a weight or more, as for the own rows.  A query
+ * that is NaN affects its own result (and the scores of its KV head) only.
  * With scores not NULL, scores[b, h, j] += sum over the heads of KV head h of their
  * weight w_j on own row j (fp32; the running weight that kani_cache_evict keeps by).
  *   q, out: [batch, Hq, D] (batch / head strides); caches [batch, Hk, cache_len, D]

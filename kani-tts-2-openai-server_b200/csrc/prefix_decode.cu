@@ -44,7 +44,7 @@ using prefix::Params;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kMaxSlack = 8.f;             // the running maximum may lag by this many powers of 2
-constexpr int64_t kSharedBytes = 128 << 20;  // prefix bytes, times the streams, from which it is read once
+constexpr int64_t kSharedBytes = 128 << 20;  // prefix bytes (K and V), times the streams, from which it is read once
 constexpr int64_t kLogitSmem = 32 * 1024;    // logits kept in shared memory up to this many bytes
 
 struct DecodeParams : Params {
@@ -440,9 +440,14 @@ DecodePlan plan_decode(int64_t batch, int hq, int hk, int d, int64_t cache_len, 
   if (scores && !p.logit_rows) p.logits = batch * hq * cache_len * 4;
   // The prefix in a launch of its own, for all streams, costs 3-6 us; read by every
   // stream's blocks it costs L2 bandwidth in the streams' number.  Measured (8 KV heads
-  // of 64, up to 500 own rows; own launch / read by each): 16 streams x 1024 rows
-  // (64 MB in all) 13.2 / 10.4 us, 64 x 1024 (256 MB) 19.0 / 34 us, 16 x 4096 (256 MB)
-  // 16.1 / 23.3 us, 64 x 256 (64 MB) 21.6 / 17.9 us.
+  // of 64, up to 500 own rows; own launch / read by each, us):
+  //    32 MiB in all: 16 streams x 1024 rows 11.7 / 10.4, 64 x 256 18.0 / 15.2
+  //    64 MiB: 16 x 2048 12.5 / 14.6, 32 x 1024 12.3 / 16.2, 64 x 512 18.5 / 19.7
+  //    96 MiB: 32 x 1536 12.9 / 20.6, 64 x 768 19.2 / 24.2, 128 x 384 27.7 / 29.9
+  //   128 MiB: 16 x 4096 16.2 / 23.4, 64 x 1024 19.4 / 28.9, 128 x 512 28.9 / 33.4
+  // The own launch rounds the prefix's weights to the storage type, these blocks keep
+  // them in two halves (result off by 2.1e-3 of its norm against 1.7e-3 in bf16): up to
+  // 128 MiB the closer result is kept, at 1.1 to 1.6 times the time from 64 MiB on.
   if (prefix_rows > 0 && batch * prefix_rows * hk * d * 4 >= kSharedBytes) {
     p.split = prefix::flash_split(1, batch, hq, hk, prefix_rows, kMaxParts);
     p.parts = p.split.parts;

@@ -1254,7 +1254,8 @@ def prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     """GQA decode attention of streams that share a prefix (``kani_prefix_decode_attention``).
 
     One query token per stream attends to the prefix rows, which all streams share
-    and which are read once for the batch, and to its own cache slots [0, kv_len[b]):
+    (read once for the batch from 128 MiB of their bytes times B on, and then weighted in
+    the storage type; by each stream, through L2, below), and to its own cache slots [0, kv_len[b]):
     ``decode_attention`` over the concatenation of both (optimized_decode.py:243-248
     with the prefix copied into every stream's buffer).
 
@@ -1345,7 +1346,8 @@ def prefix_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
             and its own rows up to that one; later tokens' outputs are zeros.
         prefix_k, prefix_v, prefix_len, scale, err_flag: as in
             ``prefix_decode_attention``.  out: optional contiguous [B, T, Hq, D].
-    Returns out [B, T, Hq, D].
+    Returns out [B, T, Hq, D].  (No scores: rows that only prompt tokens have looked at
+    have none, so ``evict_cache`` keeps them by ``protect`` or lets them go first.)
     """
     (index, code, b, t, hq, hk, d, qb, qt, qh, cb, ch, cs, s_len, ph, ps, rows, expanded) = _once(
         _check_prefix_prefill, q, k_cache, v_cache, kv_len, prefix_k, prefix_v, prefix_len, q_len, out, err_flag)
