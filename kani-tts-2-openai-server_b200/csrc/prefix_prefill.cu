@@ -57,9 +57,9 @@ template <int D> struct FlashShape {
   static constexpr int kStages = D == 64 ? 4 : 2;
   // One pair of weights in so many by polynomial instead of the special-function unit,
   // which takes 8 cycles for a warp's 32: with D = 64 that unit is the busiest (4 x 4096
-  // tokens behind 4096 rows: none 610 us, one in 4 565, one in 6 552, one in 8 557 before
-  // rows moved their maxima alone, 560 with it), with
-  // D = 128 the products weigh twice as much (3 x 777 tokens: none 55.7 us, one in 4 58.0).
+  // tokens behind 4096 rows: none 589 us, one in 4 568, one in 6 562, one in 8 563), with
+  // D = 128 the products weigh twice as much (3 x 777 tokens: none 53.8-55.8 us, one in 4
+  // 54.3-54.4, between runs on one GPU and on several: no gain).
   static constexpr int kFmaOneIn = D == 64 ? 6 : 0;
   static constexpr uint32_t kQBytes = kRows * D * 2;
   static constexpr uint32_t kTileBytes = kKeys * D * 2;

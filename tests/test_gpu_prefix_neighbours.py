@@ -110,3 +110,37 @@ def test_streams_of_one_batch(dtype, rise, what, b):
         ref, mass, dot, _ = O.prefix_decode_attention(q.view(b, 1, D), k, v, lens, pk[:, seen], pv[:, seen],
                                                       int(seen.sum()), 1.0)
         check_out(out[odd], ref[odd, 0], mass[odd, 0], dot[odd, 0], p + 9, 6.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq,hk,d", [(8, 1, 64), (6, 2, 128)])
+def test_heads_of_one_group(hq, hk, d, dtype):
+    """A NaN query head beside the others of its group: the group's heads are rows of one
+    product, in the streams' own rows and in the prompt pass."""
+    g = torch.Generator().manual_seed(93)
+    b, p, s = 5, 130, 200
+    q = make((b, hq, d), g, dtype)
+    pk, pv = make((hk, p, d), g, dtype), make((hk, p, d), g, dtype)
+    k, v = make((b, hk, s, d), g, dtype), make((b, hk, s, d), g, dtype)
+    lens = [200, 0, 64, 17, 129]
+    odd = [1, hq - 1]
+    live = [h for h in range(hq) if h not in odd]
+    bad = q.clone()
+    bad[:, odd] = float("nan")
+    rest = [x.to(DEV) for x in (k, v, torch.tensor(lens), pk, pv)]
+    ref, mass, dot, add = O.prefix_decode_attention(q, k, v, lens, pk, pv, p, d ** -0.5)
+    scores = torch.zeros(b, hk, s, device=DEV)
+    out = K.prefix_decode_attention(bad.to(DEV), *rest, scores=scores)
+    assert out[:, odd].isnan().all()
+    check_out(out[:, live], ref[:, live], mass[:, live], dot[:, live], p + s, 6.0)
+    t = 9
+    q4 = make((b, t, hq, d), g, dtype)
+    lens = [200, 9, 64, 17, 129]
+    rest[2] = torch.tensor(lens, device=DEV)
+    ref, mass, dot = O.prefix_prefill_attention(q4, k, v, lens, [t] * b, pk, pv, p, d ** -0.5)
+    bad4 = q4.clone()
+    bad4[:, :, odd] = float("nan")
+    clean, out = (K.prefix_prefill_attention(x.to(DEV), *rest) for x in (q4, bad4))
+    check_out(clean, ref, mass, dot, p + s, 6.0)
+    assert out[:, :, odd].isnan().all()
+    assert torch.equal(out[:, :, live], clean[:, :, live])
